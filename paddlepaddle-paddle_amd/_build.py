@@ -54,8 +54,11 @@ def build_kernels(verbose=False, jobs=None):
         objs.append(o)
         if _newer(s, o, headers):
             todo.append((s, o))
+    # no packed fp32 instructions (v_pk_add/mul/fma_f32, which -O3 forms from ordinary float code): some of
+    # their forms have given wrong results on this hardware
     cmds = [[HIPCC, '-O3', f'--offload-arch={ARCH}', '-fPIC', '-std=c++17', '-ffp-contract=fast', '-munsafe-fp-atomics',
-             '-I', CSRC, '-c', s, '-o', o] for s, o in todo]
+             '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-I', CSRC, '-c', s, '-o', o]
+            for s, o in todo]
     jobs = jobs or min(8, os.cpu_count() or 4)
     with concurrent.futures.ThreadPoolExecutor(jobs) as ex:
         for out in ex.map(_run, cmds):
