@@ -1,0 +1,591 @@
+// Attention over a paged KV cache for a batch that shares a prefix: o = softmax([prefix keys, own keys])
+// [prefix values, own values], the prefix read once for all sequences.
+//
+// Mathematics.  A softmax over a union of key sets joins from its parts: with (m, l, a) = (max, sum of
+// exp(s - m), sum of exp(s - m) v) of each part, m* = max m, o = sum a exp(m - m*) / sum l exp(m - m*).
+// So the work is cut into items, each a tile of query rows against a range of keys:
+//   * prefix items: the rows of a key head are ALL its query rows (T tokens x G query heads of the group),
+//     cut into tiles of 16 RTP rows; the keys are one range of the shared prefix;
+//   * own items: the rows are one sequence's (its n new tokens x G), in tiles of 16 RTO rows; the keys one
+//     range of its own pages, up to and including each row's own token (bottom-right causal).
+// An item writes (m, l, a) in 32 bits; a second kernel joins a row's items in a fixed order (no atomics).
+//
+// A block is one item: NW waves, each with a contiguous part of the item's keys and its own stage in LDS,
+// so no barrier stands in the key loop.  A wave streams 32-key tiles of K and V by LDS-DMA, the next tile
+// in flight while it computes on this one.  S^T = K Q^T on v_mfma_f32_16x16x32 (a lane holds 4 + 4 keys of
+// one row: maximum and sum take two lane swaps), P stays in registers as the B operand of O^T = V^T P^T,
+// whose A operand is V read transposed (ds_read_b64_tr_b16) in the matching key order.  P is rounded to
+// the inputs' type for that product, with a maximum that lags by at most 2^8 (no overflow in fp16), sums
+// and accumulators are 32-bit.  The NW parts are joined in LDS at the end.
+//
+// Keys past the range and keys of unallocated pages (table entries outside the cache) are read from a row
+// of zeros and masked: what lies in a page's unused slots never reaches a product.
+#define PA_FA_PAIR_GROUP_DECL static __constant__
+#include "flash_attn_kernels.h"
+
+namespace pa {
+namespace pfx {
+
+using fa::f32x4;
+using fa::s16x8;
+
+__device__ const uint16_t g_zero_row[256] __attribute__((aligned(16))) = {0};
+
+struct Args {
+  const uint16_t* q;
+  const uint16_t* kc;
+  const uint16_t* vc;
+  long long qt, qh;            // token / head strides of q
+  long long cb, ch, cr;        // block / head / slot strides of both caches
+  const int* tables;           // [B, max_blocks]
+  long long tstride;
+  const int* ptable;           // [pblocks]
+  const int* plen_dev;
+  const int* lens;
+  const int* cu;
+  uint16_t* out;               // [T, Hq, D]
+  float* lse;                  // [T, Hq] or null
+  float* wa;                   // [slots, T Hq, D]
+  float2* wml;                 // [slots, T Hq]
+  int max_blocks, pblocks, plen, num_blocks, page, page_shift;
+  int T, B, Hq, Hkv, G;
+  int ntp, nsp, nto, nso;      // row tiles and key ranges of the two kinds
+  int most;                    // new tokens of a sequence at most
+  float scale;                 // log2 units
+};
+
+// Keys per range when `len` keys are cut into at most n ranges: a multiple of 32 keys a wave, and no range
+// shorter than two tiles a wave (a shorter one costs more to join than to read).
+__host__ __device__ __forceinline__ int range_keys(int len, int n, int nw) {
+  const int per = (int)(((long long)len + n - 1) / n), unit = 32 * nw;
+  const int r = (per + unit - 1) / unit * unit;
+  return r < 2 * unit ? 2 * unit : r;
+}
+
+__device__ __forceinline__ int prefix_len(const Args& A) {
+  const long long cap = (long long)A.pblocks * A.page;
+  const int p = A.plen_dev ? *A.plen_dev : A.plen;
+  return p < 0 ? 0 : (int)min((long long)p, cap);
+}
+__device__ __forceinline__ int own_len(const Args& A, int b) {
+  const long long cap = (long long)A.max_blocks * A.page;
+  const int p = A.lens[b];
+  return p < 0 ? 0 : (int)min((long long)p, cap);
+}
+
+// One 16-B-per-lane LDS-DMA from a per-lane 64-bit address (fa_glds takes a base that all lanes share)
+__device__ __forceinline__ void glds64(const void* src, unsigned lds_dst) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(src), "s"(lds_dst)
+      : "memory");
+}
+
+// Weight of a part (m, l) in a join to maximum M.  A part that saw no key has m = -inf and l = 0; one whose
+// scores were all NaN has m = -inf and l = NaN, which has to reach the result.
+__device__ __forceinline__ float part_weight(float2 ml, float M) {
+  return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : NAN) : fa::fast_exp2(ml.x - M);
+}
+// 1 / l; 0 for a row that saw no key; NaN stays NaN
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : NAN); }
+__device__ __forceinline__ float row_lse(float M, float l) {
+  return l > 0.f ? (M + __builtin_amdgcn_logf(l)) * fa::kLn2 : (l == 0.f ? -INFINITY : NAN);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// v of the other 16-lane rows: max / sum over the four lane groups g = lane >> 4 of a column
+__device__ __forceinline__ float groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// Pages of a wave's key range: 64 table entries in a register, one per lane
+struct Window {
+  const int* table;
+  int count, w0, val;
+  __device__ __forceinline__ void load(int p) {
+    w0 = p;
+    const int i = p + (int)(threadIdx.x & 63);
+    val = i < count ? table[i] : -1;
+  }
+  __device__ __forceinline__ int at(int p) const { return __builtin_amdgcn_readlane(val, p - w0); }        // uniform p
+  __device__ __forceinline__ int at_lane(int p) const { return __shfl(val, p - w0, 64); }
+};
+
+template <typename T, int D, int NW>
+struct Shared {
+  static constexpr int TILE = 32 * D * 2;       // bytes of 32 keys
+  static constexpr int STAGE = 4 * TILE;        // K and V, two buffers
+  static constexpr int RPI = 1024 / (D * 2);    // rows of one DMA instruction
+  static constexpr int NI = 32 / RPI;           // DMA instructions of a tile
+  static constexpr int OP = D + 4;              // row pitch of the joined accumulators (floats)
+};
+template <int RT, int D, int NW>
+constexpr int lds_bytes() {
+  constexpr int stage = NW * 4 * 32 * D * 2, join = NW * RT * 16 * (D + 4) * 4;
+  return (stage > join ? stage : join) + NW * RT * 16 * 8;
+}
+
+// One item: rows [row0, row0 + 16 RT) of `nrows` rows (row r = token tok0 + r / G, head hk G + r % G)
+// against keys [k0, k1) of `table`; row r sees keys < lim0 + r / G (CAUSAL) or all.
+template <typename T, int D, int RT, int NW, bool CAUSAL>
+__device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0, int row0, int nrows, int k0, int k1,
+                                     const int* table, int tcount, int lim0, int slot, bool direct) {
+  using SH = Shared<T, D, NW>;
+  constexpr int KS = D / 32, DB = D / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+
+  // queries: B operand of S^T, lane holds Q[row c16][32 ks + 8 g .. + 8]
+  s16x8 qf[RT][KS];
+  int lim[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = row0 + 16 * t + c16, i = r / A.G;
+    lim[t] = r < nrows ? (CAUSAL ? lim0 + i : k1) : 0;
+    const uint16_t* p = A.q + (long long)(tok0 + i) * A.qt + (long long)(hk * A.G + r % A.G) * A.qh + 8 * g;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      qf[t][k] = r < nrows ? *reinterpret_cast<const s16x8*>(p + 32 * k) : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+  // the first key that some row of the tile does not see
+  const int full = CAUSAL ? lim0 + row0 / A.G : k1;
+
+  f32x4 acc[RT][DB];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // this wave's keys
+  const int per = ((k1 - k0 + NW - 1) / NW + 31) / 32 * 32;
+  const int ka = min(k0 + wave * per, k1), kb = min(ka + per, k1);
+  const int nt = (kb - ka + 31) / 32;
+  char* const st = smem + wave * SH::STAGE;
+  const unsigned st32 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)st;
+  const int rl = lane / (D / 8), cl = lane % (D / 8);  // row of a DMA instruction, chunk that this lane writes
+  const uint16_t* const kh = A.kc + hk * A.ch;
+  const uint16_t* const vh = A.vc + hk * A.ch;
+  auto page_of = [&](int key) { return A.page_shift >= 0 ? key >> A.page_shift : key / A.page; };
+
+  Window win{table, tcount, 0, -1};
+  if (nt > 0) win.load(page_of(ka));
+
+  // tile of keys [kt, kt + 32) -> stage `buf`: 2 NI DMA instructions on every path.  Returns the lanes' keys
+  // (key kt + lane, lanes 0 .. 31) that exist.
+  auto issue = [&](int kt, int buf) -> unsigned {
+    const int p1 = page_of(min(kt + 31, kb - 1));
+    if (p1 - win.w0 >= 64) win.load(page_of(kt));
+    const int key = kt + (lane & 31);
+    const int blk_l = win.at_lane(min(page_of(key), p1));
+    const unsigned ok = (unsigned)__ballot(key < kb && (unsigned)blk_l < (unsigned)A.num_blocks);
+    const unsigned dk = __builtin_amdgcn_readfirstlane(st32 + buf * 2 * SH::TILE), dv = dk + SH::TILE;
+    if (ok == 0xffffffffu && A.page % SH::RPI == 0) {
+      // whole tile, the rows of an instruction in one page: a scalar base each
+#pragma unroll
+      for (int i = 0; i < SH::NI; ++i) {
+        const int k = kt + i * SH::RPI, p = page_of(k);
+        const long long o = win.at(p) * A.cb + (k - p * A.page) * A.cr;
+        const int row = i * SH::RPI + rl;
+        fa::fa_glds(kh + o, (unsigned)(rl * (int)A.cr * 2 + ((cl ^ fa::swz_b128<D>(row)) << 4)), dk + i * 1024);
+        fa::fa_glds(vh + o, (unsigned)(rl * (int)A.cr * 2 + ((cl ^ fa::swz_tr<D>(row)) << 4)), dv + i * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < SH::NI; ++i) {
+        const int row = i * SH::RPI + rl, k = kt + row, p = page_of(k);
+        const bool have = (ok >> row) & 1;
+        const long long o = (long long)win.at_lane(min(p, p1)) * A.cb + (long long)(k - p * A.page) * A.cr;
+        const int ck = (cl ^ fa::swz_b128<D>(row)) * 8, cv = (cl ^ fa::swz_tr<D>(row)) * 8;
+        glds64(have ? kh + o + ck : g_zero_row + ck, dk + i * 1024);
+        glds64(have ? vh + o + cv : g_zero_row + cv, dv + i * 1024);
+      }
+    }
+    return ok;
+  };
+
+  unsigned ok = nt > 0 ? issue(ka, 0) : 0;
+  for (int it = 0; it < nt; ++it) {
+    const int kt = ka + 32 * it;
+    const unsigned here = ok;
+    if (it + 1 < nt) {
+      ok = issue(kt + 32, (it + 1) & 1);
+      wait_vm<2 * SH::NI>();
+    } else {
+      wait_vm<0>();
+    }
+    const char* const kbuf = st + (it & 1) * 2 * SH::TILE;
+    const char* const vbuf = kbuf + SH::TILE;
+
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const s16x8 a0 = fa::ld_row8<D, false>(kbuf, c16, k, g);
+      const s16x8 a1 = fa::ld_row8<D, false>(kbuf, 16 + c16, k, g);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        s[t][0] = fa::Mfma<T>::run(a0, qf[t][k], s[t][0]);
+        s[t][1] = fa::Mfma<T>::run(a1, qf[t][k], s[t][1]);
+      }
+    }
+    if (here != 0xffffffffu || kt + 32 > full) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 16 * h + 4 * g + e;
+            if (!((here >> r) & 1) || kt + r >= lim[t]) s[t][h][e] = -INFINITY;
+          }
+    }
+    s16x8 pf[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                       fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+      mx = groups_max(mx) * A.scale;
+      // the base of the exponents moves only when the maximum outgrows it by 2^8
+      const bool move = mx > m[t] + fa::kRescaleTau;
+      if (__ballot(move)) {
+        const float mn = move ? mx : m[t];
+        const float f = move ? fa::fast_exp2(m[t] - mn) : 1.f;  // first keys of a row: exp2(-inf) = 0
+        m[t] = mn;
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[t][d] *= f;
+      }
+      const float mb = m[t] == -INFINITY ? 0.f : m[t];  // no key seen yet: every exponent is -inf
+      float p[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[h][e] = fa::fast_exp2(s[t][h][e] * A.scale - mb);
+          l[t] += p[h][e];
+        }
+      unsigned w[4];
+      w[0] = fa::f2s2<T>(p[0][0], p[0][1]);
+      w[1] = fa::f2s2<T>(p[0][2], p[0][3]);
+      w[2] = fa::f2s2<T>(p[1][0], p[1][1]);
+      w[3] = fa::f2s2<T>(p[1][2], p[1][3]);
+      pf[t] = __builtin_bit_cast(s16x8, w);
+    }
+    bool odd = false;
+    if constexpr (CAUSAL) {
+      // a tile that some rows see in part: its values may hold an infinity or a NaN of a later token, which
+      // a zero probability in a product would carry into the earlier tokens' rows
+      if (kt + 32 > full) {
+        constexpr unsigned EX = __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
+        for (int i = lane; i < SH::TILE / 16; i += 64) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vbuf + i * 16);
+          const unsigned w4[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) odd |= (w4[j] & EX) == EX || ((w4[j] >> 16) & EX) == EX;
+        }
+      }
+      odd = __ballot(odd) != 0;
+      if (odd) {
+        // the finite values in one product; which rows meet an infinity or a NaN, in three more
+        constexpr short ONE = __is_same(T, f16_t) ? 0x3c00 : 0x3f80, INF = __is_same(T, f16_t) ? 0x7c00 : 0x7f80;
+#pragma unroll 1
+        for (int kind = 0; kind < 4; ++kind) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const bool inf = (v[j] & 0x7fff) == INF, nan = (v[j] & 0x7fff) > INF;
+              const bool is = kind == 1 ? inf && v[j] > 0 : (kind == 2 ? inf && v[j] < 0 : nan);
+              v[j] = kind == 0 ? (inf || nan ? (short)0 : v[j]) : (is ? ONE : (short)0);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+              const f32x4 z = fa::Mfma<T>::run(v, pf[t], f32x4{0.f, 0.f, 0.f, 0.f});
+              const float hit = kind == 1 ? INFINITY : (kind == 2 ? -INFINITY : NAN);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[t][d][e] += kind == 0 ? z[e] : (z[e] > 0.f ? hit : 0.f);
+            }
+          }
+        }
+      }
+    }
+    if (!odd) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t][d] = fa::Mfma<T>::run(v, pf[t], acc[t][d]);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer is written again by the next issue
+  }
+
+  // join the waves' parts
+  float2* const ml = reinterpret_cast<float2*>(smem + lds_bytes<RT, D, NW>() - NW * RT * 16 * 8);
+  float* const oj = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    l[t] = groups_sum(l[t]);
+    if (g == 0) ml[(wave * RT + t) * 16 + c16] = make_float2(m[t], l[t]);
+  }
+  __syncthreads();  // every wave is past its stage
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[(w * RT + t) * 16 + c16].x);
+    const float f = part_weight(make_float2(m[t], l[t]), M);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      *reinterpret_cast<f32x4*>(oj + ((wave * RT + t) * 16 + c16) * SH::OP + 16 * d + 4 * g) = acc[t][d] * f;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < RT * 16 * (D / 4); i += NW * 64) {
+    const int rr = i / (D / 4), d = (i % (D / 4)) * 4, r = row0 + rr;
+    if (r >= nrows) continue;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w * RT * 16 + rr].x);
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float2 x = ml[w * RT * 16 + rr];
+      L += x.y * part_weight(x, M);
+      o += *reinterpret_cast<const f32x4*>(oj + (w * RT * 16 + rr) * SH::OP + d);
+    }
+    const long long row = (long long)(tok0 + r / A.G) * A.Hq + hk * A.G + r % A.G;
+    if (direct) {
+      const float k = inverse_sum(L);
+      if (L == 0.f) o = f32x4{0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<uint2*>(A.out + row * D + d) = make_uint2(fa::f2s2<T>(o[0] * k, o[1] * k), fa::f2s2<T>(o[2] * k, o[3] * k));
+      if (A.lse && d == 0) A.lse[row] = row_lse(M, L);
+    } else {
+      *reinterpret_cast<f32x4*>(A.wa + ((long long)slot * A.T * A.Hq + row) * D + d) = o;
+      if (d == 0) A.wml[(long long)slot * A.T * A.Hq + row] = make_float2(M, L);
+    }
+  }
+}
+
+__device__ __forceinline__ void seq_rows(const Args& A, int b, int& tok0, int& n) {
+  tok0 = A.cu ? A.cu[b] : b;
+  n = A.cu ? A.cu[b + 1] - tok0 : 1;
+  if (tok0 < 0 || n < 0 || tok0 + n > A.T || n > A.most) n = 0;  // offsets that do not fit the call: nothing is read
+}
+
+// Items in the order of dispatch: groups of 8 blocks (one per XCD) of prefix and own items in turn, so that
+// the prefix's products and the own pages' stream share the chip; each XCD has a contiguous part of the
+// items, whose row tiles over the same keys are neighbours and meet in its L2.
+template <typename T, int D, int RTP, int RTO, int NW>
+__global__ __launch_bounds__(NW * 64, 1) void items_kernel(Args A) {
+  constexpr int RTM = RTP > RTO ? RTP : RTO;
+  __shared__ __attribute__((aligned(16))) char smem[lds_bytes<RTM, D, NW>()];
+  const int np = A.Hkv * A.ntp * A.nsp, no = A.B * A.Hkv * A.nto * A.nso;
+  const int gp = (np + 7) / 8, go = (no + 7) / 8, x = blockIdx.x & 7;
+  int j = blockIdx.x >> 3;
+  const int both = 2 * min(gp, go);
+  bool prefix;
+  if (j < both) {
+    prefix = (j & 1) == 0;
+    j >>= 1;
+  } else {
+    prefix = gp > go;
+    j -= both / 2;
+  }
+  const bool direct = A.wa == nullptr;
+  if (prefix) {
+    const int id = x * gp + j;
+    if (id >= np) return;
+    const int tile = id % A.ntp, sp = id / A.ntp % A.nsp, hk = id / (A.ntp * A.nsp);
+    const int len = prefix_len(A), r = range_keys(len, A.nsp, NW);
+    const int k0 = min((long long)sp * r, (long long)len), k1 = min(k0 + r, len);
+    if (k0 >= k1 && !direct) return;  // the join skips it too
+    item<T, D, RTP, NW, false>(A, smem, hk, 0, tile * 16 * RTP, A.T * A.G, k0, k1, A.ptable, A.pblocks, 0, sp, direct);
+  } else {
+    const int id = x * go + j;
+    if (id >= no) return;
+    const int tile = id % A.nto, sp = id / A.nto % A.nso, hk = id / (A.nto * A.nso) % A.Hkv,
+              b = id / (A.nto * A.nso) / A.Hkv;
+    int tok0, n;
+    seq_rows(A, b, tok0, n);
+    const int row0 = tile * 16 * RTO;
+    if (row0 >= n * A.G) return;
+    const int len = own_len(A, b), r = range_keys(len, A.nso, NW);
+    const int lim0 = len - n + 1;  // keys that the first new token sees
+    const int last = min(len, lim0 + (min(row0 + 16 * RTO, n * A.G) - 1) / A.G);
+    const int k0 = min((long long)sp * r, (long long)len), k1 = max(k0, min(k0 + r, last));
+    if (k0 >= len && !direct) return;
+    item<T, D, RTO, NW, true>(A, smem, hk, tok0, row0, n * A.G, k0, k1, A.tables + (long long)b * A.tstride,
+                              A.max_blocks, lim0, A.nsp + sp, direct);
+  }
+}
+
+// Join of a row's items: one wave a row.  A row behind the last sequence, and a row that sees no key, is
+// zero (lse -inf).  A row of a sequence that brings more tokens than the call allows is NaN.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void join_kernel(Args A, int nw) {
+  constexpr int E = D / 64;
+  const long long rows = (long long)A.T * A.Hq;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63, t = (int)(row / A.Hq);
+  int b;
+  bool over = false;
+  if (A.cu) {
+    int lo = -1, hi = A.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (A.cu[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    b = t < A.cu[A.B] ? lo : -1;
+    if (b >= 0) {
+      int tok0, n;
+      seq_rows(A, b, tok0, n);
+      over = A.cu[b + 1] - tok0 > A.most;
+      if (n == 0) b = -1;
+    }
+  } else {
+    b = t < A.B ? t : -1;
+  }
+  const int pl = b >= 0 ? prefix_len(A) : 0, ol = b >= 0 ? own_len(A, b) : 0;
+  const int rp = range_keys(pl, A.nsp > 0 ? A.nsp : 1, nw), ro = range_keys(ol, A.nso > 0 ? A.nso : 1, nw);
+  const int ap = A.nsp > 0 ? (pl + rp - 1) / rp : 0, ao = A.nso > 0 ? (ol + ro - 1) / ro : 0;
+  float M = -INFINITY;
+  for (int s = 0; s < ap + ao; ++s) M = fmaxf(M, A.wml[(s < ap ? s : A.nsp + s - ap) * rows + row].x);
+  float L = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int s = 0; s < ap + ao; ++s) {
+    const long long i = (s < ap ? s : A.nsp + s - ap) * rows + row;
+    const float2 x = A.wml[i];
+    const float f = part_weight(x, M);
+    L += x.y * f;
+    float a[E];
+    load_f<float, E>(A.wa + i * D + lane * E, a);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += a[e] * f;
+  }
+  if (over) L = NAN;
+  const float k = inverse_sum(L);
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = L == 0.f ? 0.f : o[e] * k;
+  store_f<T, E>(reinterpret_cast<T*>(A.out) + row * D + lane * E, o);
+  if (A.lse && lane == 0) A.lse[row] = row_lse(M, L);
+}
+
+template <typename T, int D, int RTP, int RTO, int NW>
+static hipError_t launch(const Args& A, hipStream_t st) {
+  static_assert(lds_bytes<(RTP > RTO ? RTP : RTO), D, NW>() <= 160 * 1024, "LDS of a block");
+  const long long np = (long long)A.Hkv * A.ntp * A.nsp, no = (long long)A.B * A.Hkv * A.nto * A.nso;
+  const long long grid = 8 * ((np + 7) / 8 + (no + 7) / 8);
+  if (np > 0x3fffffff || no > 0x3fffffff || grid > 0x7fffffff) return hipErrorInvalidValue;
+  if (grid > 0) items_kernel<T, D, RTP, RTO, NW><<<(int)grid, NW * 64, 0, st>>>(A);
+  if (A.wa) {
+    const long long rows = (long long)A.T * A.Hq;
+    join_kernel<T, D><<<(int)((rows + 3) / 4), 256, 0, st>>>(A, NW);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace pfx
+}  // namespace pa
+
+using namespace pa::pfx;
+
+// Head dims and waves of a block
+static int pfx_nw(int D) { return D == 256 ? 2 : 4; }
+
+// Row tiles of 16 an item holds: one where 16 rows hold them all, else as many as the registers do (the own
+// items' masks take some of them)
+static int pfx_rtp(long long rows, int D) { return rows <= 16 ? 1 : (D == 256 ? 2 : 4); }
+static int pfx_rto(long long rows, int D) { return rows <= 16 ? 1 : 256 / D; }
+
+// The cut of a call (`packed`: queries by offsets): out[0..3] = row tiles and key ranges (prefix, own), out[4] = slots (0: no workspace).
+// `plen` / `own`: upper bounds of the prefix's and a sequence's length (the tables' capacity when the
+// lengths are on the device).
+PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, int packed, long long plen,
+                                long long own, int* out) {
+  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || most <= 0 || (D != 64 && D != 128 && D != 256))
+    return (int)hipErrorInvalidValue;
+  const long long G = Hq / Hkv, nw = pfx_nw(D);
+  const int rtp = pfx_rtp((long long)T * G, D), rto = pfx_rto(most * G, D);
+  const long long ntp = (T * G + 16 * rtp - 1) / (16 * rtp), nto = (most * G + 16 * rto - 1) / (16 * rto);
+  auto ranges = [&](long long len, long long items, long long target) -> long long {
+    if (len <= 0) return 0;
+    const long long cap = (len + 64 * nw - 1) / (64 * nw);  // two tiles a wave at least
+    long long n = (target + items - 1) / items;
+    const long long floor_ = (len + 8191) / 8192;           // no block walks more than 8192 keys alone
+    if (n < floor_) n = floor_;
+    return n < 1 ? 1 : (n > cap ? cap : n);
+  };
+  // two blocks a CU of each kind
+  out[0] = (int)ntp;
+  out[1] = (int)ranges(plen, Hkv * ntp, 512);
+  out[2] = (int)nto;
+  long long no = ranges(own, (long long)B * Hkv * nto, 512);
+  out[3] = (int)no;
+  if (out[1] + out[3] == 0) out[3] = 1;
+  // one range for every row: written straight to the output; not with packed queries, of which some rows may
+  // belong to no sequence and are the join's to clear
+  out[4] = out[1] + out[3] == 1 && !packed ? 0 : out[1] + out[3];
+  return 0;
+}
+
+PA_API int pa_prefix_attn(const void* q, const void* kc, const void* vc, long long qt, long long qh,
+                          const long long* cstr, const int* tables, long long tstride, int max_blocks,
+                          const int* ptable, int pblocks, const int* plen_dev, int plen, int num_blocks, int page,
+                          const int* lens, const int* cu, void* out, float* lse, float* wa, float* wml,
+                          const int* plan, int T, int B, int Hq, int Hkv, int D, int most, float scale, int dt,
+                          hipStream_t st) {
+  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || page <= 0 || num_blocks < 0 || (dt != 1 && dt != 2) ||
+      !(scale > 0.f) || cstr[2] > (1 << 27) || (!cu && T != B) || (plan[4] > 0 && (!wa || !wml)))
+    return (int)hipErrorInvalidValue;
+  Args A;
+  A.q = (const uint16_t*)q; A.kc = (const uint16_t*)kc; A.vc = (const uint16_t*)vc;
+  A.qt = qt; A.qh = qh; A.cb = cstr[0]; A.ch = cstr[1]; A.cr = cstr[2];
+  A.tables = tables; A.tstride = tstride; A.max_blocks = max_blocks;
+  A.ptable = ptable; A.pblocks = pblocks; A.plen_dev = plen_dev; A.plen = plen;
+  A.lens = lens; A.cu = cu;
+  A.out = (uint16_t*)out; A.lse = lse; A.wa = plan[4] > 0 ? wa : nullptr; A.wml = (float2*)wml; A.most = most;
+  A.num_blocks = num_blocks; A.page = page;
+  A.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
+  A.T = T; A.B = B; A.Hq = Hq; A.Hkv = Hkv; A.G = Hq / Hkv;
+  A.ntp = plan[0]; A.nsp = plan[1]; A.nto = plan[2]; A.nso = plan[3];
+  A.scale = scale * pa::fa::kLog2e;
+  const int rtp = pfx_rtp((long long)T * A.G, D), rto = pfx_rto((long long)most * A.G, D);
+#define PA_PFX(TT, DD, BIG, NW)                                                        \
+  if (D == DD) {                                                                       \
+    if (256 / DD > 1 && rto > 1) return (int)launch<TT, DD, BIG, 256 / DD, NW>(A, st); \
+    if (rtp > 1) return (int)launch<TT, DD, BIG, 1, NW>(A, st);                        \
+    return (int)launch<TT, DD, 1, 1, NW>(A, st);                                       \
+  }
+#define PA_PFX_T(TT)        \
+  PA_PFX(TT, 64, 4, 4)      \
+  PA_PFX(TT, 128, 4, 4)     \
+  PA_PFX(TT, 256, 2, 2)
+  if (dt == 1) {
+    PA_PFX_T(pa::bf16_t)
+  } else {
+    PA_PFX_T(pa::f16_t)
+  }
+#undef PA_PFX_T
+#undef PA_PFX
+  return (int)hipErrorInvalidValue;
+}

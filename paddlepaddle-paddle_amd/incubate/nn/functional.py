@@ -923,3 +923,237 @@ def fused_ec_moe(x, gate, bmm0_weight, bmm0_bias, bmm1_weight, bmm1_bias, act_ty
 
 def blha_get_max_len(seq_lens_encoder, seq_lens_decoder, batch_size):
     return _w(_u(seq_lens_encoder).max().reshape(1)), _w(_u(seq_lens_decoder).max().reshape(1))
+
+
+# ------------------------------------------------------- a serving step over a paged KV cache
+def _check(ok, name, what):
+    if not ok:
+        raise ValueError(f"{name}: {what}")
+
+
+def _same_device(name, first, **others):
+    for k, t in others.items():
+        if isinstance(t, torch.Tensor) and t.device != first.device:
+            raise ValueError(f"{name}: {k} is on {t.device}, the input on {first.device}")
+
+
+def _int32(name, what, t, shape):
+    t = _u(t)
+    _check(isinstance(t, torch.Tensor) and t.dtype in (torch.int32, torch.int64), name, f"{what} must be an integer tensor")
+    _check(t.dim() == len(shape) and all(n is None or n == m for n, m in zip(shape, t.shape)), name,
+           f"{what} must have shape {list(shape)}, got {list(t.shape)}")
+    return t.to(torch.int32).contiguous()
+
+
+def _frequencies(name, inv_freq, D, interleaved):
+    f = _u(inv_freq)
+    _check(isinstance(f, torch.Tensor) and f.dim() == 1 and f.dtype in (torch.float32, torch.float64), name,
+           "inv_freq must be a one-dimensional float32 or float64 tensor")
+    _check(2 * f.numel() <= D and f.numel() <= ops.rotary_paged.MAX_PAIRS, name,
+           f"{f.numel()} frequencies turn {2 * f.numel()} values of a head: it has {D}, and at most "
+           f"{2 * ops.rotary_paged.MAX_PAIRS} can be turned")
+    _check(not interleaved or D % 2 == 0, name, f"interleaved pairs need an even head dim, got {D}")
+    return f
+
+
+def rotary_inv_freq(rotary_dim, base=10000.0, scaling=None):
+    """Angles per position of the rotary_dim / 2 pairs, for positions past the trained length, and the factor
+    that goes onto the rotated values: (inv_freq float64 [rotary_dim / 2], attention_scale), to be handed to
+    ``fused_partial_rotary_embedding`` and ``paged_rotary_append``.
+
+    ``scaling`` is None (inv_freq[i] = base ** (-2 i / rotary_dim)) or a dict with ``type`` and ``factor``:
+    ``linear`` divides every frequency by the factor; ``ntk`` raises the base to base * factor **
+    (rotary_dim / (rotary_dim - 2)); ``wavelength`` keeps pairs that make at least ``high_freq_factor`` (4) turns
+    over ``original_max_position``, divides those under ``low_freq_factor`` (1) turns and blends between them by
+    the number of turns; ``yarn`` blends by the pair's index between the pairs of ``beta_fast`` (32) and
+    ``beta_slow`` (1) turns, and scales the rotated values by 0.1 ln(factor) + 1 (``attention_factor``
+    overrides it)."""
+    name = 'rotary_inv_freq'
+    R = int(rotary_dim)
+    _check(R > 0 and R % 2 == 0, name, f"rotary_dim must be even and positive, got {rotary_dim}")
+    _check(base > 0, name, f"base must be positive, got {base}")
+    i = torch.arange(0, R, 2, dtype=torch.float64) / R
+    f, out_scale = float(base) ** -i, 1.0
+    if scaling is not None:
+        kind, factor = scaling.get('type'), float(scaling.get('factor', 1.0))
+        _check(factor > 0, name, f"factor must be positive, got {factor}")
+        if kind == 'linear':
+            f = f / factor
+        elif kind == 'ntk':
+            _check(R > 2, name, "ntk scaling needs rotary_dim > 2")
+            f = (float(base) * factor ** (R / (R - 2))) ** -i
+        elif kind in ('wavelength', 'yarn'):
+            _check(scaling.get('original_max_position', 0) > 0, name, f"{kind} scaling needs original_max_position")
+            span = float(scaling['original_max_position'])
+            if kind == 'wavelength':
+                lo, hi = float(scaling.get('low_freq_factor', 1.0)), float(scaling.get('high_freq_factor', 4.0))
+                _check(hi > lo, name, "high_freq_factor must be above low_freq_factor")
+                keep = ((span * f / (2 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
+            else:
+                def pair(turns):
+                    return R * math.log(span / (turns * 2 * math.pi)) / (2 * math.log(base))
+                lo = max(math.floor(pair(float(scaling.get('beta_fast', 32.0)))), 0)
+                hi = min(math.ceil(pair(float(scaling.get('beta_slow', 1.0)))), R - 1)
+                keep = 1.0 - ((torch.arange(R // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+                out_scale = float(scaling.get('attention_factor', 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
+            f = f * keep + f / factor * (1.0 - keep)
+        else:
+            raise ValueError(f"{name}: unknown scaling type {kind!r} (linear, ntk, wavelength, yarn)")
+    from ...core.place import current_device
+    return _w(f.to(current_device())), out_scale
+
+
+def fused_partial_rotary_embedding(q, k=None, inv_freq=None, position_ids=None, interleaved=False,
+                                   attention_scale=1.0):
+    """Rotary position embedding of the first 2 * len(inv_freq) values of each head; the rest is copied.
+
+    q [B, S, Hq, D] and k [B, S, Hkv, D] (or packed tokens, [T, H, D]; strided views are read in place), of one
+    type (float32, float16, bfloat16); inv_freq [pairs] float64 or float32 (``rotary_inv_freq``); position_ids
+    integers [B, S], [1, S] or [S] ([T] for packed tokens), default 0 .. S - 1.  Pair i is (x[i], x[i + pairs]),
+    or (x[2 i], x[2 i + 1]) with ``interleaved``; it is turned by position * inv_freq[i] and multiplied by
+    ``attention_scale``.  Angles are formed in 64 bits, so positions may be far beyond a table's length, and no
+    table is built; both tensors take one kernel, and the gradient one more.  Returns (q, k), contiguous
+    (k None if not given)."""
+    name = 'fused_partial_rotary_embedding'
+    a, b = _u(q), _u(k) if k is not None else None
+    _check(a.dim() in (3, 4), name, f"q must be [B, S, H, D] or [T, H, D], got {list(a.shape)}")
+    _check(a.dtype in ops.rotary_paged.FLOATS, name, f"unsupported type {a.dtype}")
+    f = _frequencies(name, inv_freq, a.shape[-1], interleaved)
+    _same_device(name, a, k=b, inv_freq=f, position_ids=_u(position_ids))
+    if b is not None:
+        _check(b.dtype == a.dtype, name, f"q is {a.dtype}, k {b.dtype}")
+        _check(b.dim() == a.dim() and b.shape[:-2] == a.shape[:-2] and b.shape[-1] == a.shape[-1], name,
+               f"k must be like q but for its heads, got {list(b.shape)} beside {list(a.shape)}")
+    packed = a.dim() == 3
+    if packed:
+        a, b = a[None], None if b is None else b[None]
+    B, S = a.shape[:2]
+    pos = None
+    if position_ids is not None:
+        pos = _u(position_ids)
+        _check(pos.dtype in (torch.int32, torch.int64), name, "position_ids must be integers")
+        pos = pos[None] if pos.dim() == 1 else pos
+        _check(pos.dim() == 2 and pos.shape[0] in (1, B) and pos.shape[1] == S, name,
+               f"position_ids must be [{B}, {S}], [1, {S}] or [{S}], got {list(_u(position_ids).shape)}")
+        pos = pos.expand(B, S)
+    yq, yk = ops.rotary_paged.rope_freq(a, b, f, pos, bool(interleaved), float(attention_scale))
+    if packed:
+        yq, yk = yq[0], None if yk is None else yk[0]
+    return _w(yq), None if yk is None else _w(yk)
+
+
+def _paged_caches(name, key_cache, value_cache):
+    kc, vc = _u(key_cache), _u(value_cache)
+    _check(kc.dim() == 4 and vc.shape == kc.shape, name, "caches must be [num_blocks, kv_heads, block_size, head_dim] "
+           f"of one shape, got {list(kc.shape)} and {list(vc.shape)}")
+    _check(vc.dtype == kc.dtype, name, f"key cache is {kc.dtype}, value cache {vc.dtype}")
+    _check(kc.stride(3) == 1 and vc.stride() == kc.stride(), name, "caches need equal strides and a unit inner stride")
+    _check(kc.shape[1] > 0 and kc.shape[2] > 0, name, "caches need at least one head and one place in a block")
+    return kc, vc
+
+
+def paged_rotary_append(qkv, key_cache, value_cache, block_tables, seq_lens, cu_seqlens_q=None, inv_freq=None,
+                        interleaved=False, attention_scale=1.0, qkv_bias=None, position_offset=0):
+    """Append a step's keys and values to a paged cache, rotating queries and keys on the way: one kernel between
+    the fused projection and the attention.
+
+    qkv [T, (Hq + 2 Hkv) * D] (rows may be strided): each token's query heads, key heads, value heads;
+    key_cache / value_cache [num_blocks, Hkv, block_size, D], written in place; block_tables [B, n] integers, the
+    blocks of each sequence in order; seq_lens [B], the tokens each sequence has in the cache before this call;
+    cu_seqlens_q [B + 1], the rows of each sequence's new tokens (default: one token each, T == B).  New token i
+    of sequence b goes to place seq_lens[b] + i; its queries and keys are turned (``fused_partial_rotary_embedding``)
+    at position place + ``position_offset`` (an int, or a one-element integer tensor: the length of a shared
+    prefix that lies before every sequence).  Without inv_freq nothing is turned.  ``qkv_bias`` is added first.
+
+    Returns (q [T, Hq, D], key_cache, value_cache).  A token whose place lies past the table, or in a block that
+    is not one of the cache's (-1), is not stored; q rows behind the last sequence are zero.  Two new tokens must
+    not share a place.  Inference only: no gradient flows."""
+    name = 'paged_rotary_append'
+    t = _u(qkv)
+    kc, vc = _paged_caches(name, key_cache, value_cache)
+    D, Hkv = kc.shape[3], kc.shape[1]
+    _check(t.dtype in ops.rotary_paged.FLOATS and t.dtype == kc.dtype, name,
+           f"qkv and caches must share a floating type, got {t.dtype} and {kc.dtype}")
+    _check(t.dim() == 2 and t.shape[1] % D == 0 and t.shape[1] // D >= 2 * Hkv, name,
+           f"qkv must be [T, (Hq + {2 * Hkv}) * {D}], got {list(t.shape)}")
+    tables = _int32(name, 'block_tables', block_tables, (None, None))
+    B = tables.shape[0]
+    lens = _int32(name, 'seq_lens', seq_lens, (B,))
+    cu = None if cu_seqlens_q is None else _int32(name, 'cu_seqlens_q', cu_seqlens_q, (B + 1,))
+    _check(cu is not None or t.shape[0] == B, name, f"{t.shape[0]} tokens for {B} sequences need cu_seqlens_q")
+    _check(tables.shape[1] > 0 or B == 0, name, "block_tables has no columns")
+    f = None if inv_freq is None else _frequencies(name, inv_freq, D, interleaved)
+    bias = None
+    if qkv_bias is not None:
+        bias = _u(qkv_bias)
+        _check(bias.numel() == t.shape[1], name, f"qkv_bias must have {t.shape[1]} values, got {bias.numel()}")
+        bias = bias.reshape(-1).to(t.dtype).contiguous()
+    off = _u(position_offset)
+    if isinstance(off, torch.Tensor):
+        _check(off.numel() == 1 and off.dtype in (torch.int32, torch.int64), name, "position_offset must be one integer")
+        off = off.reshape(1).to(torch.int32)
+    _same_device(name, t, key_cache=kc, value_cache=vc, block_tables=tables, seq_lens=lens, cu_seqlens_q=cu, inv_freq=f,
+                 qkv_bias=bias, position_offset=off)
+    with torch.no_grad():
+        q = ops.rotary_paged.paged_append(t.detach(), kc, vc, tables, lens, cu, f, bool(interleaved),
+                                          float(attention_scale), bias, off)
+    return _w(q), key_cache if isinstance(key_cache, Tensor) else _w(kc), \
+        value_cache if isinstance(value_cache, Tensor) else _w(vc)
+
+
+def shared_prefix_attention(query, key_cache, value_cache, block_tables, seq_lens, prefix_blocks=None, prefix_len=None,
+                            cu_seqlens_q=None, max_seqlen_q=None, scale=None, return_lse=False):
+    """Attention over a paged cache for a batch that shares a prefix, whose keys and values are read once for all
+    sequences.
+
+    query [T, Hq, D]: the new tokens of all sequences, one each or ``cu_seqlens_q`` [B + 1] with at most
+    ``max_seqlen_q`` of a sequence (an int; default T); key_cache / value_cache [num_blocks, Hkv, block_size, D];
+    block_tables [B, n], seq_lens [B]: each sequence's own blocks and keys, its new tokens' included.
+    prefix_blocks [m], prefix_len: the shared prefix's blocks and keys (an int, or a one-element integer tensor; default
+    all of the blocks' places).  New token i of n sees the whole prefix and its sequence's keys up to its own, j <=
+    seq_lens[b] - n + i.  scale defaults to 1 / sqrt(D).
+
+    Returns out [T, Hq, D], or (out, lse [T, Hq] float32) with ``return_lse``.  A token that sees no key, and a row
+    behind the last sequence, is zero (lse -inf).  Keys in blocks that are not the cache's (-1) are not seen, lengths
+    past a table are cut to it, rows of a sequence with more than max_seqlen_q tokens are NaN.  The kernel takes
+    float16 and bfloat16 with head dims 64, 128 and 256; other inputs take the composite of elementary operations,
+    which waits for the device.  Inference only: no gradient flows."""
+    name = 'shared_prefix_attention'
+    q = _u(query)
+    kc, vc = _paged_caches(name, key_cache, value_cache)
+    _check(q.dim() == 3 and q.shape[2] == kc.shape[3], name,
+           f"query must be [T, heads, {kc.shape[3]}], got {list(q.shape)}")
+    _check(q.dtype in ops.rotary_paged.FLOATS and q.dtype == kc.dtype, name,
+           f"query and caches must share a floating type, got {q.dtype} and {kc.dtype}")
+    _check(q.shape[1] % kc.shape[1] == 0, name, f"{q.shape[1]} query heads do not divide over {kc.shape[1]} key heads")
+    tables = _int32(name, 'block_tables', block_tables, (None, None))
+    B = tables.shape[0]
+    lens = _int32(name, 'seq_lens', seq_lens, (B,))
+    cu = None if cu_seqlens_q is None else _int32(name, 'cu_seqlens_q', cu_seqlens_q, (B + 1,))
+    _check(cu is not None or q.shape[0] == B, name, f"{q.shape[0]} queries for {B} sequences need cu_seqlens_q")
+    most = 1 if cu is None else (q.shape[0] if max_seqlen_q is None else int(max_seqlen_q))
+    _check(most >= 1 or q.shape[0] == 0, name, f"max_seqlen_q must be positive, got {max_seqlen_q}")
+    pt, pl = None, 0
+    if prefix_blocks is not None:
+        pt = _int32(name, 'prefix_blocks', prefix_blocks, (None,))
+        pl = _u(prefix_len)
+        if pl is None:
+            pl = pt.numel() * kc.shape[2]
+        elif isinstance(pl, torch.Tensor):
+            _check(pl.numel() == 1 and pl.dtype in (torch.int32, torch.int64), name, "prefix_len must be one integer")
+            pl = pl.reshape(1).to(torch.int32)
+        else:
+            _check(0 <= int(pl) <= pt.numel() * kc.shape[2], name,
+                   f"prefix_len {pl} does not fit {pt.numel()} blocks of {kc.shape[2]}")
+    else:
+        _check(prefix_len is None or not isinstance(_u(prefix_len), torch.Tensor) and int(prefix_len) == 0, name,
+               "prefix_len without prefix_blocks")
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
+    _check(scale > 0 and math.isfinite(scale), name, f"scale must be positive and finite, got {scale}")
+    aligned = kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in kc.stride()[:3])
+    _check(aligned or not ops.prefix_attn.supported(q, kc, vc), name, "caches need 16-byte aligned rows")
+    _same_device(name, q, key_cache=kc, value_cache=vc, block_tables=tables, seq_lens=lens, cu_seqlens_q=cu,
+                 prefix_blocks=pt, prefix_len=pl)
+    with torch.no_grad():
+        o, lse = ops.prefix_attn.attend(q.detach(), kc, vc, tables, lens, pt, pl, cu, most, scale, bool(return_lse))
+    return (_w(o), _w(lse)) if return_lse else _w(o)

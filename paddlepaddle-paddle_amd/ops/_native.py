@@ -5,6 +5,7 @@ kernels interleave correctly with the storage layer's own work and can be captur
 hipGraphs.  A failed launch raises immediately (the hipError_t is checked per call).
 """
 from ..framework.flags import pa_flag  # noqa: E402
+import contextlib
 import ctypes
 import os
 
@@ -23,6 +24,8 @@ LL = ctypes.c_longlong
 F = ctypes.c_float
 U32 = ctypes.c_uint32
 LLP = ctypes.POINTER(ctypes.c_longlong)
+IP = ctypes.POINTER(ctypes.c_int)
+D = ctypes.c_double
 
 _SIGS = {
     'pa_layernorm_fwd': [P, P, P, P, P, P, P, P, I, I, F, I, I, P],
@@ -167,6 +170,12 @@ _SIGS = {
     'pa_decode_attn_q8': [I, P, LL, P, P, P, P, I, I, LL, P, P, LL, P, LL, P, I, I, I, I, I, F, P, P, LL, P],
     'pa_kv_cache_write': [I, P, P, LL, P, P, P, P, P, I, I, LL, P, P, I, I, I, P],
     'pa_kv_cache_write_q8': [I, I, P, P, LL, P, P, P, I, I, LL, P, P, I, I, I, P, P, LL, I, F, F, P],
+    'pa_rope_freq': [P, P, P, P, LLP, LLP, I, I, I, I, I, I, I, P, F, P, LL, LL, I, F, I, I, P],
+    'pa_paged_append': [P, LL, P, P, P, P, LLP, P, LL, I, I, I, P, P, P, LL, I, I, I, I, I, I, I, P, F, P, P, LL, I, I,
+                        I, P],
+    'pa_prefix_attn_plan': [I, I, I, I, I, I, I, LL, LL, IP],
+    'pa_prefix_attn': [P, P, P, LL, LL, LLP, P, LL, I, P, I, P, I, I, I, P, P, P, P, P, P, IP, I, I, I, I, I, I, F, I, P],
+    'pa_sample': [P, LL, I, I, P, I, P, P, P, P, D, I, D, D, P, P, I, P],
     'pa_flash_fwd': [P, P, P, P, P, I, I, I, I, I, I, LLP, LLP, LLP, LLP, F, I, I, P],
     'pa_flash_bwd': [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, LLP, LLP, LLP, LLP, LLP, LLP, LLP, LLP, F, I, I,
                      P],
@@ -211,6 +220,13 @@ def check(err, name):
 
 def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def device_of(t):
+    """Context in which launches go to the device that holds ``t`` (which may not be the current one)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def ptr(t):

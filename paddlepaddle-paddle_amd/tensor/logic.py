@@ -139,6 +139,46 @@ def top_p_sampling(x, ps, threshold=None, topp_seed=None, seed=-1, k=0, mode='tr
     return _w(probs.gather(-1, ids)), _w(ids)
 
 
+def filtered_sampling(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, name=None):
+    """One token per row of logits x [rows, vocab], from given random numbers ``uniform`` [rows] (or [rows, 1]) in
+    [0, 1), after temperature, top-k, top-p and min-p; every setting is a number or a tensor of one per row.
+
+    Of the tokens in the order of falling logits (equal ones: the lower index first) the first ``top_k`` are kept (0:
+    all), of those the ones before which less than ``top_p`` of their mass lies (1: all; at least one), of those the
+    ones with at least ``min_p`` of the largest probability (0: all).  The answer is the first token, in the order of
+    the vocabulary, at which the kept mass passes uniform times its total.  A temperature of 0 takes the largest logit
+    (the lowest index of equal ones).  Tokens of -inf and NaN are never taken; a row that has no other gives token -1
+    and probability 0.  Sums are 64-bit: the answer does not depend on the device or on the order of addition.
+
+    Returns (probs float32, ids int64), both [rows, 1]: the tokens and their shares of the kept mass.  Inference
+    only: no gradient flows.  Beside ``top_p_sampling`` (probabilities in, its own random numbers)."""
+    from .. import ops
+    t, u = _u(x), _u(uniform)
+    if t.dim() != 2 or t.shape[1] == 0 or t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"filtered_sampling: x must be [rows, vocab] in float32, float16 or bfloat16, got {t.dtype} "
+                         f"{list(t.shape)}")
+    if not isinstance(u, torch.Tensor) or not u.is_floating_point() or u.numel() != t.shape[0]:
+        raise ValueError(f"filtered_sampling: uniform must be a floating tensor of {t.shape[0]} numbers")
+
+    def setting(v, what, whole=False):
+        v = _u(v)
+        if not isinstance(v, torch.Tensor):
+            return int(v) if whole else float(v)
+        if v.numel() != t.shape[0] or v.is_floating_point() == whole:
+            raise ValueError(f"filtered_sampling: {what} must be a number or {t.shape[0]} "
+                             f"{'integers' if whole else 'floating numbers'}, got {v.dtype} {list(v.shape)}")
+        if v.device != t.device:
+            raise ValueError(f"filtered_sampling: {what} is on {v.device}, x on {t.device}")
+        return v.reshape(-1)
+    if u.device != t.device:
+        raise ValueError(f"filtered_sampling: uniform is on {u.device}, x on {t.device}")
+    settings = (setting(temperature, 'temperature'), setting(top_k, 'top_k', True), setting(top_p, 'top_p'),
+                setting(min_p, 'min_p'))
+    with torch.no_grad():
+        probs, ids = ops.sampling.sample(t.detach(), u.detach().reshape(-1), *settings)
+    return _w(probs), _w(ids)
+
+
 # ----------------------------------------------------------------------------- stat
 def var(x, axis=None, unbiased=True, keepdim=False, name=None):
     t = _u(x)
