@@ -24,6 +24,12 @@ OBJ = os.path.join(LIB, 'obj')
 ARCH = os.environ.get('PADDLE_AMD_ARCH', 'gfx950')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 
+FILE_FLAGS = {
+    # matrix instructions with vector-register accumulators: a wave of this kernel owns the whole register file, and
+    # accumulators in its upper half are moved to the lower one and back in every turn of the key loop
+    'prefix_attn.hip': ['-mllvm', '-amdgpu-mfma-vgpr-form=1'],
+}
+
 KERNEL_LIB = os.path.join(LIB, 'libpaddle_amd_kernels.so')
 RUNTIME_LIB = os.path.join(LIB, 'libpaddle_amd_runtime.so')
 ALLOC_LIB = os.path.join(LIB, 'libpaddle_amd_alloc.so')
@@ -58,7 +64,7 @@ def build_kernels(verbose=False, jobs=None):
     # their forms have given wrong results on this hardware
     cmds = [[HIPCC, '-O3', f'--offload-arch={ARCH}', '-fPIC', '-std=c++17', '-ffp-contract=fast', '-munsafe-fp-atomics',
              '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-I', CSRC, '-c', s, '-o', o]
-            for s, o in todo]
+            + FILE_FLAGS.get(os.path.basename(s), []) for s, o in todo]
     jobs = jobs or min(8, os.cpu_count() or 4)
     with concurrent.futures.ThreadPoolExecutor(jobs) as ex:
         for out in ex.map(_run, cmds):

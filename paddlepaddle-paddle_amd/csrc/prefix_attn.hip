@@ -94,19 +94,43 @@ __device__ __forceinline__ float row_lse(float M, float l) {
   return l > 0.f ? (M + __builtin_amdgcn_logf(l)) * fa::kLn2 : (l == 0.f ? -INFINITY : NAN);
 }
 
+// The N DMA instructions of a tile whose rows lie in one page: instruction i writes 1 KiB at dst + 1024 i from
+// base + off[i] + 1024 (i % 4).  The instruction's own offset moves both ends, so M0 changes every fourth time.
+template <int N>
+__device__ __forceinline__ void dma_tile(const char* base, const unsigned (&off)[N], unsigned dst) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    unsigned keep;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %5\n\t"
+        "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+        "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+        "global_load_lds_dwordx4 %4, %5 offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(off[i]), "v"(off[i + 1]), "v"(off[i + 2]), "v"(off[i + 3]), "s"(base), "s"(dst + i * 1024)
+        : "memory");
+  }
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// v of the other 16-lane rows: max / sum over the four lane groups g = lane >> 4 of a column
-__device__ __forceinline__ float groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
-__device__ __forceinline__ float groups_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+
+// maximum over the four lane groups g = lane >> 4 of a column
+__device__ __forceinline__ float groups_max(float v) {
+  // lane swaps instead of two trips through LDS; s_nop: a VALU result is read by a lane swap
+  float a = v, b = v;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  a = b = fmaxf(a, b);
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return fmaxf(a, b);
 }
 
 // Pages of a wave's key range: 64 table entries in a register, one per lane
@@ -117,23 +141,24 @@ struct Window {
     w0 = p;
     const int i = p + (int)(threadIdx.x & 63);
     val = i < count ? table[i] : -1;
+    // waited for here, where it is rare: at its uses the compiler's wait would drain the tiles in flight too
+    asm volatile("s_waitcnt vmcnt(0)" : "+v"(val)::"memory");
   }
-  __device__ __forceinline__ int at(int p) const { return __builtin_amdgcn_readlane(val, p - w0); }        // uniform p
-  __device__ __forceinline__ int at_lane(int p) const { return __shfl(val, p - w0, 64); }
+  __device__ __forceinline__ int at(int p) const { return __shfl(val, p - w0, 64); }
 };
 
 template <typename T, int D, int NW>
 struct Shared {
   static constexpr int TILE = 32 * D * 2;       // bytes of 32 keys
-  static constexpr int STAGE = 4 * TILE;        // K and V, two buffers
+  static constexpr int STAGE = 2 * TILE;        // K and V
   static constexpr int RPI = 1024 / (D * 2);    // rows of one DMA instruction
   static constexpr int NI = 32 / RPI;           // DMA instructions of a tile
   static constexpr int OP = D + 4;              // row pitch of the joined accumulators (floats)
 };
 template <int RT, int D, int NW>
 constexpr int lds_bytes() {
-  constexpr int stage = NW * 4 * 32 * D * 2, join = NW * RT * 16 * (D + 4) * 4;
-  return (stage > join ? stage : join) + NW * RT * 16 * 8;
+  constexpr int stage = NW * 2 * 32 * D * 2, join = NW * 16 * (D + 4) * 4;
+  return (stage > join ? stage : join) + NW * RT * 16 * 8 + RT * 16 * D;
 }
 
 // One item: rows [row0, row0 + 16 RT) of `nrows` rows (row r = token tok0 + r / G, head hk G + r % G)
@@ -161,76 +186,112 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
   // the first key that some row of the tile does not see
   const int full = CAUSAL ? lim0 + row0 / A.G : k1;
 
-  f32x4 acc[RT][DB];
-  float m[RT], l[RT];
+  f32x4 acc[RT][DB];            // O^T
+  float l[RT];                  // sum of this lane's probabilities, before they are rounded
+  float nm[RT], thr[RT];        // minus the base of the exponents; the score at which it has to move
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    m[t] = -INFINITY;
+    nm[t] = 0.f;
+    thr[t] = -INFINITY;
     l[t] = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // LDS: the waves' stages, later the parts to be joined; (m, l) of each wave and row; what of a row's values
+  // was not finite (bits 0, 1, 2 of a byte: +inf, -inf, NaN)
+  float2* const ml = reinterpret_cast<float2*>(smem + lds_bytes<RT, D, NW>() - NW * RT * 16 * 8 - RT * 16 * D);
+  unsigned* const notes = reinterpret_cast<unsigned*>(smem + lds_bytes<RT, D, NW>() - RT * 16 * D);
+  if constexpr (CAUSAL) {
+    for (int i = threadIdx.x; i < RT * 16 * D / 4; i += NW * 64) notes[i] = 0;
+    __syncthreads();
   }
 
   // this wave's keys
   const int per = ((k1 - k0 + NW - 1) / NW + 31) / 32 * 32;
   const int ka = min(k0 + wave * per, k1), kb = min(ka + per, k1);
   const int nt = (kb - ka + 31) / 32;
-  char* const st = smem + wave * SH::STAGE;
-  const unsigned st32 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)st;
+  char* const st = smem + wave * SH::STAGE;  // K, V
+  const unsigned st32 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)st);
   const int rl = lane / (D / 8), cl = lane % (D / 8);  // row of a DMA instruction, chunk that this lane writes
-  const uint16_t* const kh = A.kc + hk * A.ch;
-  const uint16_t* const vh = A.vc + hk * A.ch;
+  const char* const kh = reinterpret_cast<const char*>(A.kc + hk * A.ch);
+  const char* const vh = reinterpret_cast<const char*>(A.vc + hk * A.ch);
   auto page_of = [&](int key) { return A.page_shift >= 0 ? key >> A.page_shift : key / A.page; };
 
   Window win{table, tcount, 0, -1};
   if (nt > 0) win.load(page_of(ka));
 
-  // tile of keys [kt, kt + 32) -> stage `buf`: 2 NI DMA instructions on every path.  Returns the lanes' keys
-  // (key kt + lane, lanes 0 .. 31) that exist.
-  auto issue = [&](int kt, int buf) -> unsigned {
+  // LDS-DMA of the 32 keys (or values) from kt on into the LDS image at dst: NI instructions on every path.
+  // A lane fetches chunk cl ^ swizzle of its row; the swizzle is that of the image.  Returns the keys (bit r:
+  // key kt + r) that exist.
+  const bool whole_page = A.page % 32 == 0 && A.cr >= D, grouped = A.page % SH::RPI == 0;
+  unsigned fk[SH::NI], fv[SH::NI];  // byte offsets of the fast path, less what the instruction's offset adds
+#pragma unroll
+  for (int i = 0; i < SH::NI; ++i) {
+    const int row = i * SH::RPI + rl;
+    const unsigned r = (unsigned)(row * (int)A.cr * 2 - (i & 3) * 1024);
+    fk[i] = r + ((unsigned)(cl ^ fa::swz_b128<D>(row)) << 4);
+    fv[i] = r + ((unsigned)(cl ^ fa::swz_tr<D>(row)) << 4);
+  }
+  auto slow = [&](auto isv, int kt, unsigned dst) -> unsigned {
+    const char* const base = isv ? vh : kh;
     const int p1 = page_of(min(kt + 31, kb - 1));
     if (p1 - win.w0 >= 64) win.load(page_of(kt));
-    const int key = kt + (lane & 31);
-    const int blk_l = win.at_lane(min(page_of(key), p1));
-    const unsigned ok = (unsigned)__ballot(key < kb && (unsigned)blk_l < (unsigned)A.num_blocks);
-    const unsigned dk = __builtin_amdgcn_readfirstlane(st32 + buf * 2 * SH::TILE), dv = dk + SH::TILE;
-    if (ok == 0xffffffffu && A.page % SH::RPI == 0) {
-      // whole tile, the rows of an instruction in one page: a scalar base each
+    const int key = kt + (lane & 31), pg = min(page_of(key), p1), blk = win.at(pg);
+    const unsigned ok = (unsigned)__ballot(key < kb && (unsigned)blk < (unsigned)A.num_blocks);
+    const unsigned long long off = (unsigned long long)((long long)blk * A.cb + (long long)(key - pg * A.page) * A.cr) * 2;
+    const unsigned lo = (unsigned)off, hi = (unsigned)(off >> 32);
+    if (ok == 0xffffffffu && grouped) {  // the rows of an instruction lie in one page: a scalar base for each
 #pragma unroll
       for (int i = 0; i < SH::NI; ++i) {
-        const int k = kt + i * SH::RPI, p = page_of(k);
-        const long long o = win.at(p) * A.cb + (k - p * A.page) * A.cr;
+        // (unsigned): readlane gives an int, whose sign would reach the upper half
+        const unsigned long long o = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(lo, i * SH::RPI) |
+                                     (unsigned long long)(unsigned)__builtin_amdgcn_readlane(hi, i * SH::RPI) << 32;
         const int row = i * SH::RPI + rl;
-        fa::fa_glds(kh + o, (unsigned)(rl * (int)A.cr * 2 + ((cl ^ fa::swz_b128<D>(row)) << 4)), dk + i * 1024);
-        fa::fa_glds(vh + o, (unsigned)(rl * (int)A.cr * 2 + ((cl ^ fa::swz_tr<D>(row)) << 4)), dv + i * 1024);
+        const unsigned sw = (unsigned)(cl ^ (isv ? fa::swz_tr<D>(row) : fa::swz_b128<D>(row))) << 4;
+        fa::fa_glds(base + o, (unsigned)(rl * (int)A.cr * 2) + sw, dst + i * 1024);
       }
-    } else {
+    } else {  // an address for each lane; rows that do not exist come from a row of zeros
 #pragma unroll
       for (int i = 0; i < SH::NI; ++i) {
-        const int row = i * SH::RPI + rl, k = kt + row, p = page_of(k);
-        const bool have = (ok >> row) & 1;
-        const long long o = (long long)win.at_lane(min(p, p1)) * A.cb + (long long)(k - p * A.page) * A.cr;
-        const int ck = (cl ^ fa::swz_b128<D>(row)) * 8, cv = (cl ^ fa::swz_tr<D>(row)) * 8;
-        glds64(have ? kh + o + ck : g_zero_row + ck, dk + i * 1024);
-        glds64(have ? vh + o + cv : g_zero_row + cv, dv + i * 1024);
+        const int row = i * SH::RPI + rl;
+        const unsigned long long o = (unsigned long long)(unsigned)__shfl((int)lo, row, 64) |
+                                     (unsigned long long)(unsigned)__shfl((int)hi, row, 64) << 32;
+        const unsigned sw = (unsigned)(cl ^ (isv ? fa::swz_tr<D>(row) : fa::swz_b128<D>(row))) << 4;
+        glds64(((ok >> row) & 1) ? base + o + sw : reinterpret_cast<const char*>(g_zero_row) + sw, dst + i * 1024);
       }
     }
     return ok;
   };
+  auto issue = [&](auto isv, int kt, unsigned dst) -> unsigned {
+    if (whole_page && kt + 32 <= kb) {  // 32 keys of one page
+      const int p = page_of(kt);
+      if (p - win.w0 >= 64) win.load(p);
+      const unsigned blk = __builtin_amdgcn_readlane(win.val, p - win.w0);
+      if (blk < (unsigned)A.num_blocks) {
+        const char* base = (isv ? vh : kh) + ((long long)blk * A.cb + (long long)(kt - p * A.page) * A.cr) * 2;
+        dma_tile<SH::NI>(base, isv ? fv : fk, dst);
+        return 0xffffffffu;
+      }
+    }
+    return slow(isv, kt, dst);
+  };
+  std::false_type isk;
+  std::true_type isv;
 
-  unsigned ok = nt > 0 ? issue(ka, 0) : 0;
+  const unsigned dk = st32, dv = st32 + SH::TILE;
+  const char* const kbuf = st;
+  const char* const vbuf = st + SH::TILE;
+  unsigned ok = 0;
+  if (nt > 0) {
+    ok = issue(isk, ka, dk);
+    issue(isv, ka, dv);
+  }
   for (int it = 0; it < nt; ++it) {
     const int kt = ka + 32 * it;
     const unsigned here = ok;
-    if (it + 1 < nt) {
-      ok = issue(kt + 32, (it + 1) & 1);
-      wait_vm<2 * SH::NI>();
-    } else {
-      wait_vm<0>();
-    }
-    const char* const kbuf = st + (it & 1) * 2 * SH::TILE;
-    const char* const vbuf = kbuf + SH::TILE;
-
+    const bool more = it + 1 < nt;
+    wait_vm<SH::NI>();  // K is here; V may be on its way
     f32x4 s[RT][2];
 #pragma unroll
     for (int t = 0; t < RT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -244,6 +305,8 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
         s[t][1] = fa::Mfma<T>::run(a1, qf[t][k], s[t][1]);
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read: the next may come
+    if (more) ok = issue(isk, kt + 32, dk);
     if (here != 0xffffffffu || kt + 32 > full) {
 #pragma unroll
       for (int t = 0; t < RT; ++t)
@@ -255,31 +318,39 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
             if (!((here >> r) & 1) || kt + r >= lim[t]) s[t][h][e] = -INFINITY;
           }
     }
-    s16x8 pf[RT];
+    // The base moves only when a score outgrows it by 2^8; whether one does needs no look at other lanes.
+    float over = -INFINITY, mx[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                       fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-      mx = groups_max(mx) * A.scale;
-      // the base of the exponents moves only when the maximum outgrows it by 2^8
-      const bool move = mx > m[t] + fa::kRescaleTau;
-      if (__ballot(move)) {
-        const float mn = move ? mx : m[t];
-        const float f = move ? fa::fast_exp2(m[t] - mn) : 1.f;  // first keys of a row: exp2(-inf) = 0
-        m[t] = mn;
+      // v_maximum3_f32 (a NaN stays: such a row ends as NaN whatever its base is)
+      mx[t] = max3(max3(max3(s[t][0][0], s[t][0][1], s[t][0][2]), s[t][0][3], s[t][1][0]),
+                   max3(s[t][1][1], s[t][1][2], s[t][1][3]), -INFINITY);
+      over = fmaxf(over, mx[t] * A.scale - thr[t]);  // NaN (nothing seen, nothing here) is passed over
+    }
+    if (__ballot(over > 0.f)) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float m1 = groups_max(mx[t]) * A.scale;
+        const bool mv = m1 > thr[t];
+        const float f = thr[t] == -INFINITY ? 0.f : (mv ? fa::fast_exp2(-nm[t] - m1) : 1.f);
+        if (mv) {
+          nm[t] = -m1;
+          thr[t] = m1 + fa::kRescaleTau;
+        }
         l[t] *= f;
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc[t][d] *= f;
       }
-      const float mb = m[t] == -INFINITY ? 0.f : m[t];  // no key seen yet: every exponent is -inf
+    }
+    s16x8 pf[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
       float p[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[h][e] = fa::fast_exp2(s[t][h][e] * A.scale - mb);
-          l[t] += p[h][e];
-        }
+        for (int e = 0; e < 4; ++e) p[h][e] = fa::fast_exp2(s[t][h][e] * A.scale + nm[t]);
+      l[t] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
       unsigned w[4];
       w[0] = fa::f2s2<T>(p[0][0], p[0][1]);
       w[1] = fa::f2s2<T>(p[0][2], p[0][3]);
@@ -287,6 +358,8 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
       w[3] = fa::f2s2<T>(p[1][2], p[1][3]);
       pf[t] = __builtin_bit_cast(s16x8, w);
     }
+    if (more) wait_vm<SH::NI>();  // V is here; the next K may be on its way
+    else wait_vm<0>();
     bool odd = false;
     if constexpr (CAUSAL) {
       // a tile that some rows see in part: its values may hold an infinity or a NaN of a later token, which
@@ -302,83 +375,110 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
       }
       odd = __ballot(odd) != 0;
       if (odd) {
-        // the finite values in one product; which rows meet an infinity or a NaN, in three more
+        // which rows meet an infinity or a NaN: products with 1 in their places and 0 elsewhere, noted in LDS
+        // and brought into the row at the join; the product below then takes the finite values alone
         constexpr short ONE = __is_same(T, f16_t) ? 0x3c00 : 0x3f80, INF = __is_same(T, f16_t) ? 0x7c00 : 0x7f80;
 #pragma unroll 1
-        for (int kind = 0; kind < 4; ++kind) {
+        for (int d = 0; d < DB; ++d) {
+          const s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+          unsigned note[RT];
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+          for (int t = 0; t < RT; ++t) note[t] = 0;
+#pragma unroll
+          for (int kind = 0; kind < 3; ++kind) {
+            s16x8 x;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const bool inf = (v[j] & 0x7fff) == INF, nan = (v[j] & 0x7fff) > INF;
-              const bool is = kind == 1 ? inf && v[j] > 0 : (kind == 2 ? inf && v[j] < 0 : nan);
-              v[j] = kind == 0 ? (inf || nan ? (short)0 : v[j]) : (is ? ONE : (short)0);
+              x[j] = (kind == 0 ? inf && v[j] > 0 : (kind == 1 ? inf && v[j] < 0 : nan)) ? ONE : (short)0;
             }
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-              const f32x4 z = fa::Mfma<T>::run(v, pf[t], f32x4{0.f, 0.f, 0.f, 0.f});
-              const float hit = kind == 1 ? INFINITY : (kind == 2 ? -INFINITY : NAN);
+              const f32x4 z = fa::Mfma<T>::run(x, pf[t], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[t][d][e] += kind == 0 ? z[e] : (z[e] > 0.f ? hit : 0.f);
+              for (int e = 0; e < 4; ++e) note[t] |= z[e] > 0.f ? 1u << (8 * e + kind) : 0u;
             }
           }
+#pragma unroll
+          for (int t = 0; t < RT; ++t) atomicOr(&notes[(16 * t + c16) * (D / 4) + 4 * d + g], note[t]);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int i = lane; i < SH::TILE / 4; i += 64) {
+          unsigned* const w = reinterpret_cast<unsigned*>(const_cast<char*>(vbuf)) + i;
+          const unsigned x = *w;
+          *w = ((x & 0x7fffu) >= (unsigned)INF ? 0u : x & 0xffffu) |
+               (((x >> 16) & 0x7fffu) >= (unsigned)INF ? 0u : x & 0xffff0000u);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
     }
-    if (!odd) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+    for (int d = 0; d < DB; ++d) {
+      const s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t][d] = fa::Mfma<T>::run(v, pf[t], acc[t][d]);
-      }
+      for (int t = 0; t < RT; ++t) acc[t][d] = fa::Mfma<T>::run(v, pf[t], acc[t][d]);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this buffer is written again by the next issue
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
+    if (more) issue(isv, kt + 32, dv);
   }
+  float m[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) m[t] = thr[t] == -INFINITY ? -INFINITY : -nm[t];
 
   // join the waves' parts
-  float2* const ml = reinterpret_cast<float2*>(smem + lds_bytes<RT, D, NW>() - NW * RT * 16 * 8);
   float* const oj = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    l[t] = groups_sum(l[t]);
+    l[t] += __shfl_xor(l[t], 16, 64);  // over the lane groups
+    l[t] += __shfl_xor(l[t], 32, 64);
     if (g == 0) ml[(wave * RT + t) * 16 + c16] = make_float2(m[t], l[t]);
   }
   __syncthreads();  // every wave is past its stage
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
+    if (t > 0) __syncthreads();
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[(w * RT + t) * 16 + c16].x);
     const float f = part_weight(make_float2(m[t], l[t]), M);
 #pragma unroll
     for (int d = 0; d < DB; ++d)
-      *reinterpret_cast<f32x4*>(oj + ((wave * RT + t) * 16 + c16) * SH::OP + 16 * d + 4 * g) = acc[t][d] * f;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < RT * 16 * (D / 4); i += NW * 64) {
-    const int rr = i / (D / 4), d = (i % (D / 4)) * 4, r = row0 + rr;
-    if (r >= nrows) continue;
-    float M = -INFINITY, L = 0.f;
+      *reinterpret_cast<f32x4*>(oj + (wave * 16 + c16) * SH::OP + 16 * d + 4 * g) = acc[t][d] * f;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
+      const int rr = i / (D / 4), d = (i % (D / 4)) * 4, r = row0 + 16 * t + rr;
+      if (r >= nrows) continue;
+      float Mr = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w * RT * 16 + rr].x);
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < NW; ++w) Mr = fmaxf(Mr, ml[(w * RT + t) * 16 + rr].x);
+      f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float2 x = ml[w * RT * 16 + rr];
-      L += x.y * part_weight(x, M);
-      o += *reinterpret_cast<const f32x4*>(oj + (w * RT * 16 + rr) * SH::OP + d);
-    }
-    const long long row = (long long)(tok0 + r / A.G) * A.Hq + hk * A.G + r % A.G;
-    if (direct) {
-      const float k = inverse_sum(L);
-      if (L == 0.f) o = f32x4{0.f, 0.f, 0.f, 0.f};
-      *reinterpret_cast<uint2*>(A.out + row * D + d) = make_uint2(fa::f2s2<T>(o[0] * k, o[1] * k), fa::f2s2<T>(o[2] * k, o[3] * k));
-      if (A.lse && d == 0) A.lse[row] = row_lse(M, L);
-    } else {
-      *reinterpret_cast<f32x4*>(A.wa + ((long long)slot * A.T * A.Hq + row) * D + d) = o;
-      if (d == 0) A.wml[(long long)slot * A.T * A.Hq + row] = make_float2(M, L);
+      for (int w = 0; w < NW; ++w) {
+        const float2 x = ml[(w * RT + t) * 16 + rr];
+        L += x.y * part_weight(x, Mr);
+        o += *reinterpret_cast<const f32x4*>(oj + (w * 16 + rr) * SH::OP + d);
+      }
+      if constexpr (CAUSAL) {
+        const unsigned n = notes[(16 * t + rr) * (D / 4) + d / 4];
+        if (n != 0)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (n >> (8 * e) & 1) o[e] += INFINITY;
+            if (n >> (8 * e) & 2) o[e] -= INFINITY;
+            if (n >> (8 * e) & 4) o[e] = NAN;
+          }
+      }
+      const long long row = (long long)(tok0 + r / A.G) * A.Hq + hk * A.G + r % A.G;
+      if (direct) {
+        const float k = inverse_sum(L);
+        if (L == 0.f) o = f32x4{0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<uint2*>(A.out + row * D + d) =
+            make_uint2(fa::f2s2<T>(o[0] * k, o[1] * k), fa::f2s2<T>(o[2] * k, o[3] * k));
+        if (A.lse && d == 0) A.lse[row] = row_lse(Mr, L);
+      } else {
+        *reinterpret_cast<f32x4*>(A.wa + ((long long)slot * A.T * A.Hq + row) * D + d) = o;
+        if (d == 0) A.wml[(long long)slot * A.T * A.Hq + row] = make_float2(Mr, L);
+      }
     }
   }
 }
@@ -393,20 +493,23 @@ __device__ __forceinline__ void seq_rows(const Args& A, int b, int& tok0, int& n
 // the prefix's products and the own pages' stream share the chip; each XCD has a contiguous part of the
 // items, whose row tiles over the same keys are neighbours and meet in its L2.
 template <typename T, int D, int RTP, int RTO, int NW>
-__global__ __launch_bounds__(NW * 64, 1) void items_kernel(Args A) {
+__global__ __launch_bounds__(NW * 64) void items_kernel(Args A) {
   constexpr int RTM = RTP > RTO ? RTP : RTO;
   __shared__ __attribute__((aligned(16))) char smem[lds_bytes<RTM, D, NW>()];
   const int np = A.Hkv * A.ntp * A.nsp, no = A.B * A.Hkv * A.nto * A.nso;
   const int gp = (np + 7) / 8, go = (no + 7) / 8, x = blockIdx.x & 7;
   int j = blockIdx.x >> 3;
-  const int both = 2 * min(gp, go);
+  // Two of the prefix, one own, while both last: blocks go to the four shader engines of an XCD in turn, and
+  // an order of period two would leave all the long ones on half of them.
+  const int n3 = min(gp / 2, go);
   bool prefix;
-  if (j < both) {
-    prefix = (j & 1) == 0;
-    j >>= 1;
+  if (j < 3 * n3) {
+    prefix = j % 3 != 2;
+    j = prefix ? j / 3 * 2 + j % 3 : j / 3;
   } else {
-    prefix = gp > go;
-    j -= both / 2;
+    j -= 3 * n3;
+    prefix = j < gp - 2 * n3;
+    j = prefix ? j + 2 * n3 : j - (gp - 2 * n3) + n3;
   }
   const bool direct = A.wa == nullptr;
   if (prefix) {
@@ -510,12 +613,12 @@ static hipError_t launch(const Args& A, hipStream_t st) {
 using namespace pa::pfx;
 
 // Head dims and waves of a block
-static int pfx_nw(int D) { return D == 256 ? 2 : 4; }
+static int pfx_nw(int D) { return D == 256 ? 4 : 8; }
 
 // Row tiles of 16 an item holds: one where 16 rows hold them all, else as many as the registers do (the own
 // items' masks take some of them)
-static int pfx_rtp(long long rows, int D) { return rows <= 16 ? 1 : (D == 256 ? 2 : 4); }
-static int pfx_rto(long long rows, int D) { return rows <= 16 ? 1 : 256 / D; }
+static int pfx_rtp(long long rows, int D) { return rows <= 16 ? 1 : (D == 64 ? 4 : 2); }
+static int pfx_rto(long long rows, int D) { return rows <= 16 ? 1 : (D == 256 ? 1 : 2); }
 
 // The cut of a call (`packed`: queries by offsets): out[0..3] = row tiles and key ranges (prefix, own), out[4] = slots (0: no workspace).
 // `plen` / `own`: upper bounds of the prefix's and a sequence's length (the tables' capacity when the
@@ -570,16 +673,16 @@ PA_API int pa_prefix_attn(const void* q, const void* kc, const void* vc, long lo
   A.ntp = plan[0]; A.nsp = plan[1]; A.nto = plan[2]; A.nso = plan[3];
   A.scale = scale * pa::fa::kLog2e;
   const int rtp = pfx_rtp((long long)T * A.G, D), rto = pfx_rto((long long)most * A.G, D);
-#define PA_PFX(TT, DD, BIG, NW)                                                        \
-  if (D == DD) {                                                                       \
-    if (256 / DD > 1 && rto > 1) return (int)launch<TT, DD, BIG, 256 / DD, NW>(A, st); \
-    if (rtp > 1) return (int)launch<TT, DD, BIG, 1, NW>(A, st);                        \
-    return (int)launch<TT, DD, 1, 1, NW>(A, st);                                       \
+#define PA_PFX(TT, DD, RP, RO, NW)                                               \
+  if (D == DD) {                                                                 \
+    if (RO > 1 && rto > 1) return (int)launch<TT, DD, RP, RO, NW>(A, st);        \
+    if (rtp > 1) return (int)launch<TT, DD, RP, 1, NW>(A, st);                   \
+    return (int)launch<TT, DD, 1, 1, NW>(A, st);                                 \
   }
-#define PA_PFX_T(TT)        \
-  PA_PFX(TT, 64, 4, 4)      \
-  PA_PFX(TT, 128, 4, 4)     \
-  PA_PFX(TT, 256, 2, 2)
+#define PA_PFX_T(TT)           \
+  PA_PFX(TT, 64, 4, 2, 8)      \
+  PA_PFX(TT, 128, 2, 2, 8)     \
+  PA_PFX(TT, 256, 2, 1, 4)
   if (dt == 1) {
     PA_PFX_T(pa::bf16_t)
   } else {

@@ -347,6 +347,39 @@ def test_attention_lengths_beyond_tables_and_strides(dev):
     near(whole._t, want, O.attention_bound(want, size, BF))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('page', [64, 16, 3])
+def test_offsets_beyond_32_bits(page):
+    """Pages around and behind 2^31 and 2^32 bytes of a cache, appended to and read."""
+    g = torch.Generator().manual_seed(8)
+    hq, hkv, d = 4, 1, 128
+    size = hkv * page * d * 2
+    nblk = (9 << 29) // size                                            # 4.5 GiB
+    used = [(1 << 31) // size - 1, (1 << 31) // size, (1 << 31) // size + 1, (1 << 32) // size - 1, (1 << 32) // size,
+            (1 << 32) // size + 1, nblk - 1, 0]
+    kc, vc = (torch.empty(nblk, hkv, page, d, dtype=BF, device='cuda') for _ in range(2))
+    small = torch.randn(2, len(used), hkv, page, d, generator=g).to(BF)
+    at = torch.tensor(used, device='cuda')
+    kc[at], vc[at] = small[0].cuda(), small[1].cuda()
+    table = torch.tensor([[4, 1, 6], [2, 3, 7]], dtype=torch.int32)     # indexes into `used`
+    common = torch.tensor([0, 5], dtype=torch.int32)
+    there = torch.tensor(used, dtype=torch.int32)
+    past = torch.tensor([2 * page - 1, 3 * page - 1], dtype=torch.int32)
+    qkv = torch.randn(2, (hq + 2) * d, generator=g).to(BF)
+    f = frequencies(64)
+    wq, wk, wv = O.append(qkv, small[0], small[1], table, past, None, f, False, 1.0, 2 * page)
+    q, _, _ = IF.paged_rotary_append(qkv.cuda(), kc, vc, there[table.long()].cuda(), past.cuda(), inv_freq=f.cuda(),
+                                     position_offset=2 * page)
+    step = torch.finfo(BF).eps / 2
+    near(q._t, wq, wq.abs() * step + 1e-5)
+    near(kc[at], wk, wk.abs() * step + 1e-5)
+    assert torch.equal(vc[at].cpu().double(), wv)
+    now = kc[at].cpu(), vc[at].cpu()
+    want, _, bound = O.attention(q._t.cpu(), *now, table, past + 1, common, 2 * page, None, d ** -0.5)
+    got = IF.shared_prefix_attention(q, kc, vc, there[table.long()].cuda(), (past + 1).cuda(), there[common.long()].cuda())
+    near(got._t, want, O.attention_bound(want, bound, BF))
+
+
 @pytest.mark.parametrize('dev', DEVICES)
 def test_attention_refusals(dev):
     z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device=dev)  # noqa: E731
