@@ -483,6 +483,184 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
   }
 }
 
+// A prefix item of many rows: the NW waves share each tile of 64 keys, two of which are in LDS, and have 16 RT
+// rows of their own: rows [row0, row0 + 16 RT NW) against keys [k0, k1), all of which every row sees.  In the
+// layout of item() each wave reads all of its own keys from L2, 32 rows at a time: at 2048 rows a key head that
+// is 19 TB/s of L2 reads, which bound it (518 TFLOP/s); here a tile serves 8 times as many rows.
+constexpr int kWideRT = 2;
+
+template <typename T, int D, int RT, int NW>
+__device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int row0, int nrows, int k0, int k1, int slot) {
+  using SH = Shared<T, D, NW>;
+  constexpr int KS = D / 32, DB = D / 16, TILE = 64 * D * 2, ND = 64 / SH::RPI / NW;  // DMA instructions a wave, K or V
+  static_assert(ND * SH::RPI * NW == 64, "a tile's rows divide over the waves");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  row0 += wave * 16 * RT;
+  s16x8 qf[RT][KS];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = row0 + 16 * t + c16;
+    const uint16_t* p = A.q + (long long)(r / A.G) * A.qt + (long long)(hk * A.G + r % A.G) * A.qh + 8 * g;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      qf[t][k] = r < nrows ? *reinterpret_cast<const s16x8*>(p + 32 * k) : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+  f32x4 acc[RT][DB];
+  float l[RT], nm[RT], thr[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    nm[t] = l[t] = 0.f;
+    thr[t] = -INFINITY;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int nt = (k1 - k0 + 63) / 64;
+  const unsigned st32 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)smem);
+  const int rl = lane / (D / 8), cl = lane % (D / 8);
+  const char* const kh = reinterpret_cast<const char*>(A.kc + hk * A.ch);
+  const char* const vh = reinterpret_cast<const char*>(A.vc + hk * A.ch);
+  auto page_of = [&](int key) { return A.page_shift >= 0 ? key >> A.page_shift : key / A.page; };
+  const bool grouped = A.page % SH::RPI == 0;
+  Window win{A.ptable, A.pblocks, 0, -1};
+  if (nt > 0) win.load(page_of(k0));
+  unsigned sk[ND], sv[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    const int row = (wave * ND + i) * SH::RPI + rl;
+    sk[i] = (unsigned)(cl ^ fa::swz_b128<D>(row)) << 4;
+    sv[i] = (unsigned)(cl ^ fa::swz_tr<D>(row)) << 4;
+  }
+  const unsigned rowb = (unsigned)(rl * (int)A.cr * 2);
+
+  // this wave's rows of the tile from kt on, K and V; returns which of the 64 keys exist
+  auto issue = [&](int kt, int buf) -> unsigned long long {
+    const int p1 = page_of(min(kt + 63, k1 - 1));
+    if (p1 - win.w0 >= 64) win.load(page_of(kt));  // 64 pages hold a tile
+    const int key = kt + lane, pg = min(page_of(key), p1), blk = win.at(pg);
+    const unsigned long long ok = __ballot(key < k1 && (unsigned)blk < (unsigned)A.num_blocks);
+    const unsigned long long off = (unsigned long long)((long long)blk * A.cb + (long long)(key - pg * A.page) * A.cr) * 2;
+    const unsigned lo = (unsigned)off, hi = (unsigned)(off >> 32);
+    const unsigned dk = st32 + buf * 2 * TILE + wave * ND * 1024, dv = dk + TILE;
+    if (ok == ~0ull && grouped) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const int r = (wave * ND + i) * SH::RPI;
+        const unsigned long long o = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(lo, r) |
+                                     (unsigned long long)(unsigned)__builtin_amdgcn_readlane(hi, r) << 32;
+        fa::fa_glds(kh + o, rowb + sk[i], dk + i * 1024);
+        fa::fa_glds(vh + o, rowb + sv[i], dv + i * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const int r = (wave * ND + i) * SH::RPI + rl;
+        const unsigned long long o = (unsigned long long)(unsigned)__shfl((int)lo, r, 64) |
+                                     (unsigned long long)(unsigned)__shfl((int)hi, r, 64) << 32;
+        const bool have = (ok >> r) & 1;
+        const char* z = reinterpret_cast<const char*>(g_zero_row);
+        glds64(have ? kh + o + sk[i] : z + sk[i], dk + i * 1024);
+        glds64(have ? vh + o + sv[i] : z + sv[i], dv + i * 1024);
+      }
+    }
+    return ok;
+  };
+
+  unsigned long long next = nt > 0 ? issue(k0, 0) : 0;
+  for (int it = 0; it < nt; ++it) {
+    const unsigned long long here = next;
+    wait_vm<0>();
+    __syncthreads();  // the whole tile is here, and every wave is done with the one before it
+    if (it + 1 < nt) next = issue(k0 + 64 * (it + 1), (it + 1) & 1);
+    const char* const kbuf = smem + (it & 1) * 2 * TILE;
+    const char* const vbuf = kbuf + TILE;
+    f32x4 s[RT][4];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) s[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const s16x8 a = fa::ld_row8<D, false>(kbuf, 16 * h + c16, k, g);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) s[t][h] = fa::Mfma<T>::run(a, qf[t][k], s[t][h]);
+      }
+    if (here != ~0ull) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!((here >> (16 * h + 4 * g + e)) & 1)) s[t][h][e] = -INFINITY;
+    }
+    float over = -INFINITY, mx[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      mx[t] = max3(max3(max3(s[t][0][0], s[t][0][1], s[t][0][2]), s[t][0][3], s[t][1][0]),
+                   max3(s[t][1][1], s[t][1][2], s[t][1][3]), s[t][2][0]);
+      mx[t] = max3(max3(mx[t], s[t][2][1], s[t][2][2]), max3(s[t][2][3], s[t][3][0], s[t][3][1]),
+                   max3(s[t][3][2], s[t][3][3], -INFINITY));
+      over = fmaxf(over, mx[t] * A.scale - thr[t]);
+    }
+    if (__ballot(over > 0.f)) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const float m1 = groups_max(mx[t]) * A.scale;
+        const bool mv = m1 > thr[t];
+        const float f = thr[t] == -INFINITY ? 0.f : (mv ? fa::fast_exp2(-nm[t] - m1) : 1.f);
+        if (mv) {
+          nm[t] = -m1;
+          thr[t] = m1 + fa::kRescaleTau;
+        }
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[t][d] *= f;
+      }
+    }
+    s16x8 pf[RT][2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float p[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[h][e] = fa::fast_exp2(s[t][2 * j + h][e] * A.scale + nm[t]);
+        l[t] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+        unsigned w[4];
+        w[0] = fa::f2s2<T>(p[0][0], p[0][1]);
+        w[1] = fa::f2s2<T>(p[0][2], p[0][3]);
+        w[2] = fa::f2s2<T>(p[1][0], p[1][1]);
+        w[3] = fa::f2s2<T>(p[1][2], p[1][3]);
+        pf[t][j] = __builtin_bit_cast(s16x8, w);
+      }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const s16x8 v = fa::ld_tr8<D, true>(vbuf, 32 * j, d, lane);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t][d] = fa::Mfma<T>::run(v, pf[t][j], acc[t][d]);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    l[t] += __shfl_xor(l[t], 16, 64);
+    l[t] += __shfl_xor(l[t], 32, 64);
+    const int r = row0 + 16 * t + c16;
+    if (r >= nrows) continue;
+    const long long row = (long long)slot * A.T * A.Hq + (long long)(r / A.G) * A.Hq + hk * A.G + r % A.G;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(A.wa + row * D + 16 * d + 4 * g) = acc[t][d];
+    if (g == 0) A.wml[row] = make_float2(thr[t] == -INFINITY ? -INFINITY : -nm[t], l[t]);
+  }
+}
+
 __device__ __forceinline__ void seq_rows(const Args& A, int b, int& tok0, int& n) {
   tok0 = A.cu ? A.cu[b] : b;
   n = A.cu ? A.cu[b + 1] - tok0 : 1;
@@ -492,10 +670,11 @@ __device__ __forceinline__ void seq_rows(const Args& A, int b, int& tok0, int& n
 // Items in the order of dispatch: groups of 8 blocks (one per XCD) of prefix and own items in turn, so that
 // the prefix's products and the own pages' stream share the chip; each XCD has a contiguous part of the
 // items, whose row tiles over the same keys are neighbours and meet in its L2.
+// RTP = 0: wide prefix items (of kWideRT row tiles a wave)
 template <typename T, int D, int RTP, int RTO, int NW>
 __global__ __launch_bounds__(NW * 64) void items_kernel(Args A) {
-  constexpr int RTM = RTP > RTO ? RTP : RTO;
-  __shared__ __attribute__((aligned(16))) char smem[lds_bytes<RTM, D, NW>()];
+  constexpr int RTM = RTP > RTO ? RTP : RTO, narrow = lds_bytes<RTM, D, NW>(), wide = RTP == 0 ? 2 * 2 * 64 * D * 2 : 0;
+  __shared__ __attribute__((aligned(16))) char smem[narrow > wide ? narrow : wide];
   const int np = A.Hkv * A.ntp * A.nsp, no = A.B * A.Hkv * A.nto * A.nso;
   const int gp = (np + 7) / 8, go = (no + 7) / 8, x = blockIdx.x & 7;
   int j = blockIdx.x >> 3;
@@ -519,7 +698,10 @@ __global__ __launch_bounds__(NW * 64) void items_kernel(Args A) {
     const int len = prefix_len(A), r = range_keys(len, A.nsp, NW);
     const int k0 = min((long long)sp * r, (long long)len), k1 = min(k0 + r, len);
     if (k0 >= k1 && !direct) return;  // the join skips it too
-    item<T, D, RTP, NW, false>(A, smem, hk, 0, tile * 16 * RTP, A.T * A.G, k0, k1, A.ptable, A.pblocks, 0, sp, direct);
+    if constexpr (RTP == 0)
+      wide_item<T, D, kWideRT, NW>(A, smem, hk, tile * 16 * kWideRT * NW, A.T * A.G, k0, k1, sp);
+    else
+      item<T, D, RTP, NW, false>(A, smem, hk, 0, tile * 16 * RTP, A.T * A.G, k0, k1, A.ptable, A.pblocks, 0, sp, direct);
   } else {
     const int id = x * go + j;
     if (id >= no) return;
@@ -595,7 +777,6 @@ __global__ __launch_bounds__(256) void join_kernel(Args A, int nw) {
 
 template <typename T, int D, int RTP, int RTO, int NW>
 static hipError_t launch(const Args& A, hipStream_t st) {
-  static_assert(lds_bytes<(RTP > RTO ? RTP : RTO), D, NW>() <= 160 * 1024, "LDS of a block");
   const long long np = (long long)A.Hkv * A.ntp * A.nsp, no = (long long)A.B * A.Hkv * A.nto * A.nso;
   const long long grid = 8 * ((np + 7) / 8 + (no + 7) / 8);
   if (np > 0x3fffffff || no > 0x3fffffff || grid > 0x7fffffff) return hipErrorInvalidValue;
@@ -618,6 +799,9 @@ static int pfx_nw(int D) { return D == 256 ? 4 : 8; }
 // Row tiles of 16 an item holds: one where 16 rows hold them all, else as many as the registers do (the own
 // items' masks take some of them)
 static int pfx_rtp(long long rows, int D) { return rows <= 16 ? 1 : (D == 64 ? 4 : 2); }
+// Whether the prefix items are wide: where more than half of a wide item's rows are there (fewer leave its waves
+// idle).  Packed queries or a prefix alone go the same way: the join is always there with a prefix and own keys.
+static bool pfx_wide(long long rows, int D) { return rows > 16 * kWideRT * pfx_nw(D) / 2; }
 static int pfx_rto(long long rows, int D) { return rows <= 16 ? 1 : (D == 256 ? 1 : 2); }
 
 // The cut of a call (`packed`: queries by offsets): out[0..3] = row tiles and key ranges (prefix, own), out[4] = slots (0: no workspace).
@@ -629,7 +813,8 @@ PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, i
     return (int)hipErrorInvalidValue;
   const long long G = Hq / Hkv, nw = pfx_nw(D);
   const int rtp = pfx_rtp((long long)T * G, D), rto = pfx_rto(most * G, D);
-  const long long ntp = (T * G + 16 * rtp - 1) / (16 * rtp), nto = (most * G + 16 * rto - 1) / (16 * rto);
+  const long long prow = pfx_wide((long long)T * G, D) ? 16 * kWideRT * nw : 16 * rtp;  // rows of a prefix item
+  const long long ntp = (T * G + prow - 1) / prow, nto = (most * G + 16 * rto - 1) / (16 * rto);
   auto ranges = [&](long long len, long long items, long long target) -> long long {
     if (len <= 0) return 0;
     const long long cap = (len + 64 * nw - 1) / (64 * nw);  // two tiles a wave at least
@@ -647,7 +832,7 @@ PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, i
   if (out[1] + out[3] == 0) out[3] = 1;
   // one range for every row: written straight to the output; not with packed queries, of which some rows may
   // belong to no sequence and are the join's to clear
-  out[4] = out[1] + out[3] == 1 && !packed ? 0 : out[1] + out[3];
+  out[4] = out[1] + out[3] == 1 && !packed && !(out[1] && pfx_wide((long long)T * G, D)) ? 0 : out[1] + out[3];
   return 0;
 }
 
@@ -673,8 +858,11 @@ PA_API int pa_prefix_attn(const void* q, const void* kc, const void* vc, long lo
   A.ntp = plan[0]; A.nsp = plan[1]; A.nto = plan[2]; A.nso = plan[3];
   A.scale = scale * pa::fa::kLog2e;
   const int rtp = pfx_rtp((long long)T * A.G, D), rto = pfx_rto((long long)most * A.G, D);
+  const bool wide = A.nsp > 0 && pfx_wide((long long)T * A.G, D);
 #define PA_PFX(TT, DD, RP, RO, NW)                                               \
   if (D == DD) {                                                                 \
+    if (wide && rto > 1) return (int)launch<TT, DD, 0, RO, NW>(A, st);           \
+    if (wide) return (int)launch<TT, DD, 0, 1, NW>(A, st);                       \
     if (RO > 1 && rto > 1) return (int)launch<TT, DD, RP, RO, NW>(A, st);        \
     if (rtp > 1) return (int)launch<TT, DD, RP, 1, NW>(A, st);                   \
     return (int)launch<TT, DD, 1, 1, NW>(A, st);                                 \
