@@ -489,6 +489,18 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
 // is 19 TB/s of L2 reads, which bound it (518 TFLOP/s); here a tile serves 8 times as many rows.
 constexpr int kWideRT = 2;
 
+// Asks the scheduler for N times one matrix instruction, three vector ones and an exponential behind it: the
+// matrix cores run while the wave issues the others
+template <int N>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+    __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+  }
+}
+
 template <typename T, int D, int RT, int NW>
 __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int row0, int nrows, int k0, int k1, int slot) {
   using SH = Shared<T, D, NW>;
@@ -533,78 +545,80 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
   }
   const unsigned rowb = (unsigned)(rl * (int)A.cr * 2);
 
-  // this wave's rows of the tile from kt on, K and V; returns which of the 64 keys exist
-  auto issue = [&](int kt, int buf) -> unsigned long long {
+  // Places of a tile's 64 keys: byte offset of key kt + lane from the head's base, and which keys exist
+  struct Places {
+    unsigned lo, hi;
+    unsigned long long ok;
+  };
+  auto places = [&](int kt) -> Places {
     const int p1 = page_of(min(kt + 63, k1 - 1));
     if (p1 - win.w0 >= 64) win.load(page_of(kt));  // 64 pages hold a tile
     const int key = kt + lane, pg = min(page_of(key), p1), blk = win.at(pg);
-    const unsigned long long ok = __ballot(key < k1 && (unsigned)blk < (unsigned)A.num_blocks);
     const unsigned long long off = (unsigned long long)((long long)blk * A.cb + (long long)(key - pg * A.page) * A.cr) * 2;
-    const unsigned lo = (unsigned)off, hi = (unsigned)(off >> 32);
-    const unsigned dk = st32 + buf * 2 * TILE + wave * ND * 1024, dv = dk + TILE;
-    if (ok == ~0ull && grouped) {
+    return Places{(unsigned)off, (unsigned)(off >> 32),
+                  (unsigned long long)__ballot(key < k1 && (unsigned)blk < (unsigned)A.num_blocks)};
+  };
+  // this wave's rows of a tile's K (or V)
+  auto issue = [&](const Places& p, const char* base, const unsigned (&sw)[ND], unsigned dst) {
+    dst += wave * ND * 1024;
+    if (p.ok == ~0ull && grouped) {
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
         const int r = (wave * ND + i) * SH::RPI;
-        const unsigned long long o = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(lo, r) |
-                                     (unsigned long long)(unsigned)__builtin_amdgcn_readlane(hi, r) << 32;
-        fa::fa_glds(kh + o, rowb + sk[i], dk + i * 1024);
-        fa::fa_glds(vh + o, rowb + sv[i], dv + i * 1024);
+        const unsigned long long o = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(p.lo, r) |
+                                     (unsigned long long)(unsigned)__builtin_amdgcn_readlane(p.hi, r) << 32;
+        fa::fa_glds(base + o, rowb + sw[i], dst + i * 1024);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
         const int r = (wave * ND + i) * SH::RPI + rl;
-        const unsigned long long o = (unsigned long long)(unsigned)__shfl((int)lo, r, 64) |
-                                     (unsigned long long)(unsigned)__shfl((int)hi, r, 64) << 32;
-        const bool have = (ok >> r) & 1;
-        const char* z = reinterpret_cast<const char*>(g_zero_row);
-        glds64(have ? kh + o + sk[i] : z + sk[i], dk + i * 1024);
-        glds64(have ? vh + o + sv[i] : z + sv[i], dv + i * 1024);
+        const unsigned long long o = (unsigned long long)(unsigned)__shfl((int)p.lo, r, 64) |
+                                     (unsigned long long)(unsigned)__shfl((int)p.hi, r, 64) << 32;
+        glds64(((p.ok >> r) & 1) ? base + o + sw[i] : reinterpret_cast<const char*>(g_zero_row) + sw[i], dst + i * 1024);
       }
     }
-    return ok;
   };
 
-  unsigned long long next = nt > 0 ? issue(k0, 0) : 0;
-  for (int it = 0; it < nt; ++it) {
-    const unsigned long long here = next;
-    wait_vm<0>();
-    __syncthreads();  // the whole tile is here, and every wave is done with the one before it
-    if (it + 1 < nt) next = issue(k0 + 64 * (it + 1), (it + 1) & 1);
-    const char* const kbuf = smem + (it & 1) * 2 * TILE;
-    const char* const vbuf = kbuf + TILE;
-    f32x4 s[RT][4];
+  f32x4 s[RT][4], c[RT][4];
+  float mx[RT], over = -INFINITY;
+  auto scores = [&](const char* kbuf, f32x4 (&o)[RT][4]) {
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int h = 0; h < 4; ++h) s[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 4; ++h) o[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const s16x8 a = fa::ld_row8<D, false>(kbuf, 16 * h + c16, k, g);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) s[t][h] = fa::Mfma<T>::run(a, qf[t][k], s[t][h]);
+        for (int t = 0; t < RT; ++t) o[t][h] = fa::Mfma<T>::run(a, qf[t][k], o[t][h]);
       }
-    if (here != ~0ull) {
+  };
+  auto mask = [&](unsigned long long ok, f32x4 (&o)[RT][4]) {
+    if (ok != ~0ull) {
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int h = 0; h < 4; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!((here >> (16 * h + 4 * g + e)) & 1)) s[t][h][e] = -INFINITY;
+            if (!((ok >> (16 * h + 4 * g + e)) & 1)) o[t][h][e] = -INFINITY;
     }
-    float over = -INFINITY, mx[RT];
+  };
+  auto maxima = [&](const f32x4 (&o)[RT][4]) {
+    over = -INFINITY;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      mx[t] = max3(max3(max3(s[t][0][0], s[t][0][1], s[t][0][2]), s[t][0][3], s[t][1][0]),
-                   max3(s[t][1][1], s[t][1][2], s[t][1][3]), s[t][2][0]);
-      mx[t] = max3(max3(mx[t], s[t][2][1], s[t][2][2]), max3(s[t][2][3], s[t][3][0], s[t][3][1]),
-                   max3(s[t][3][2], s[t][3][3], -INFINITY));
+      const float a = max3(max3(o[t][0][0], o[t][0][1], o[t][0][2]), o[t][0][3], o[t][1][0]);
+      const float b = max3(max3(o[t][1][1], o[t][1][2], o[t][1][3]), o[t][2][0], o[t][2][1]);
+      const float d = max3(max3(o[t][2][2], o[t][2][3], o[t][3][0]), o[t][3][1], o[t][3][2]);
+      mx[t] = max3(max3(a, b, d), o[t][3][3], o[t][3][3]);
       over = fmaxf(over, mx[t] * A.scale - thr[t]);
     }
+  };
+  auto rebase = [&] {
     if (__ballot(over > 0.f)) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
@@ -620,32 +634,111 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
         for (int d = 0; d < DB; ++d) acc[t][d] *= f;
       }
     }
-    s16x8 pf[RT][2];
+  };
+
+  // LDS: two buffers of K, two of V.  Pipeline: while a tile's probabilities are formed, the next tile's scores
+  // are on the matrix cores.
+  Places pl{0, 0, 0};
+  unsigned long long ok = 0;
+  if (nt > 0) {
+    pl = places(k0);
+    ok = pl.ok;
+    issue(pl, kh, sk, st32);
+    issue(pl, vh, sv, st32 + 2 * TILE);
+    if (nt > 1) {
+      pl = places(k0 + 64);
+      issue(pl, kh, sk, st32 + TILE);
+    }
+    wait_vm<0>();
+    __syncthreads();
+    scores(smem, s);
+    mask(ok, s);
+    maxima(s);
+    rebase();
+  }
+  for (int it = 0; it < nt; ++it) {
+    const bool more = it + 1 < nt;
+    wait_vm<0>();
+    __syncthreads();  // V of this tile and K of the next are here, and every wave is done with the ones before
+    if (more) issue(pl, vh, sv, st32 + (2 + ((it + 1) & 1)) * TILE);
+    ok = pl.ok;
+    if (it + 2 < nt) {
+      pl = places(k0 + 64 * (it + 2));
+      issue(pl, kh, sk, st32 + (it & 1) * TILE);
+    }
+    const char* const kbuf = smem + ((it + 1) & 1) * TILE;
+    const char* const vbuf = smem + (2 + (it & 1)) * TILE;
+    // Phase 1: 8 RT / 2 products a step with a part of the probabilities under them, the operands of the next
+    // step on their way from LDS; phase 2: the product with the values, four operands ahead.  The barriers keep
+    // the compiler from sinking each read to its product, where a wave would wait out the LDS's latency 48
+    // times a tile.  (Behind the last tile the scores are of stale bytes, and never used.)
+    s16x8 pf[RT][2], fr[2][4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) fr[0][h] = fa::ld_row8<D, false>(kbuf, 16 * h + c16, 0, g);
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float p[2][4];
+      for (int h = 0; h < 4; ++h) c[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+    for (int k = 0; k < KS; ++k) {
+      if (k + 1 < KS) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[h][e] = fa::fast_exp2(s[t][2 * j + h][e] * A.scale + nm[t]);
-        l[t] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
-        unsigned w[4];
-        w[0] = fa::f2s2<T>(p[0][0], p[0][1]);
-        w[1] = fa::f2s2<T>(p[0][2], p[0][3]);
-        w[2] = fa::f2s2<T>(p[1][0], p[1][1]);
-        w[3] = fa::f2s2<T>(p[1][2], p[1][3]);
-        pf[t][j] = __builtin_bit_cast(s16x8, w);
+        for (int h = 0; h < 4; ++h) fr[(k + 1) & 1][h] = fa::ld_row8<D, false>(kbuf, 16 * h + c16, k + 1, g);
+      } else {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) fr[(k + 1) & 1][d] = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
       }
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int h = 0; h < 4; ++h)
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const s16x8 v = fa::ld_tr8<D, true>(vbuf, 32 * j, d, lane);
+        for (int t = 0; t < RT; ++t) c[t][h] = fa::Mfma<T>::run(fr[k & 1][h], qf[t][k], c[t][h]);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t][d] = fa::Mfma<T>::run(v, pf[t][j], acc[t][d]);
+      for (int i = 0; i < 2 * RT; ++i)  // part i of the probabilities: row tile i / 2, 32 keys i % 2
+        if (i * KS / (2 * RT) == k) {
+          const int t = i / 2, j = i % 2;
+          float p[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[h][e] = fa::fast_exp2(s[t][2 * j + h][e] * A.scale + nm[t]);
+          l[t] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+          unsigned w[4];
+          w[0] = fa::f2s2<T>(p[0][0], p[0][1]);
+          w[1] = fa::f2s2<T>(p[0][2], p[0][3]);
+          w[2] = fa::f2s2<T>(p[1][0], p[1][1]);
+          w[3] = fa::f2s2<T>(p[1][2], p[1][3]);
+          pf[t][j] = __builtin_bit_cast(s16x8, w);
+        }
+      interleave<4 * RT>();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int q = 0; q < 2 * DB / 4; ++q) {  // operands 4 q ..: 32 keys (4 q) / DB, values (4 q) % DB ..
+      if (q + 1 < 2 * DB / 4) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int i = 4 * (q + 1) + d;
+          fr[(KS + q + 1) & 1][d] = fa::ld_tr8<D, true>(vbuf, 32 * (i / DB), i % DB, lane);
+        }
       }
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int i = 4 * q + d;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          acc[t][i % DB] = fa::Mfma<T>::run(fr[(KS + q) & 1][d], pf[t][i / DB], acc[t][i % DB]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int h = 0; h < 4; ++h) s[t][h] = c[t][h];
+    if (more) {
+      mask(ok, s);
+      maxima(s);
+      rebase();
+    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 #pragma unroll
