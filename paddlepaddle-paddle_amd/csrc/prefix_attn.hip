@@ -27,6 +27,7 @@ namespace pa {
 namespace pfx {
 
 using fa::f32x4;
+using fa::s16x4;
 using fa::s16x8;
 
 __device__ const uint16_t g_zero_row[256] __attribute__((aligned(16))) = {0};
@@ -131,6 +132,32 @@ __device__ __forceinline__ float groups_max(float v) {
   a = b = fmaxf(a, b);
   asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
   return fmaxf(a, b);
+}
+
+// Operands from the LDS images of K and V tiles, by 32-bit LDS addresses.  A lane's address in the swizzled image is
+// one constant, with the operand's number put over it by an exclusive or (the images are those of fa::lds_off).
+typedef __attribute__((address_space(3))) const char lds_char;
+template <int D>
+__device__ __forceinline__ unsigned row_base(int lane) {  // K: row lane & 15, 8 values from 8 (lane >> 4) on
+  const int r = lane & 15, sw = fa::swz_b128<D>(r);
+  return (unsigned)(r * D * 2 + ((((lane >> 4) ^ sw) & 3) << 4) + ((sw >> 2) << 6));
+}
+template <int D>
+__device__ __forceinline__ s16x8 read_row(unsigned tile, unsigned base, int h, int k) {  // rows 16 h .., values 32 k ..
+  return *(__attribute__((address_space(3))) const s16x8*)(tile + (base ^ (unsigned)(k << 6)) + (unsigned)(h * 16 * D * 2));
+}
+template <int D>
+__device__ __forceinline__ unsigned col_base(int lane) {  // V transposed: row 4 (lane >> 4) + lane / 4 % 4, columns 4 (lane % 4) ..
+  const int r = 4 * (lane >> 4) + ((lane >> 2) & 3), p = lane & 3;
+  return (unsigned)(r * D * 2 + (p >> 1) * 16 + (p & 1) * 8 + (fa::swz_tr<D>(r) << 4));
+}
+template <int D>
+__device__ __forceinline__ s16x8 read_col(unsigned tile, unsigned base, int j, int d) {  // rows 32 j .., columns 16 d ..
+  typedef __attribute__((address_space(3))) s16x4 lds_v4;
+  const unsigned at = tile + (base ^ (unsigned)(d << 5)) + (unsigned)(32 * j * D * 2);
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)at);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4*)(at + 16 * D * 2));
+  return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
 // Pages of a wave's key range: 64 table entries in a register, one per lane
@@ -252,12 +279,14 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
         fa::fa_glds(base + o, (unsigned)(rl * (int)A.cr * 2) + sw, dst + i * 1024);
       }
     } else {  // an address for each lane; rows that do not exist come from a row of zeros
+      int ln = lane;
+      asm volatile("" : "+v"(ln));  // rare: its addresses are formed here, not kept in registers through the loop
 #pragma unroll
       for (int i = 0; i < SH::NI; ++i) {
-        const int row = i * SH::RPI + rl;
+        const int row = i * SH::RPI + ln / (D / 8);
         const unsigned long long o = (unsigned long long)(unsigned)__shfl((int)lo, row, 64) |
                                      (unsigned long long)(unsigned)__shfl((int)hi, row, 64) << 32;
-        const unsigned sw = (unsigned)(cl ^ (isv ? fa::swz_tr<D>(row) : fa::swz_b128<D>(row))) << 4;
+        const unsigned sw = (unsigned)((ln % (D / 8)) ^ (isv ? fa::swz_tr<D>(row) : fa::swz_b128<D>(row))) << 4;
         glds64(((ok >> row) & 1) ? base + o + sw : reinterpret_cast<const char*>(g_zero_row) + sw, dst + i * 1024);
       }
     }
@@ -280,8 +309,8 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
   std::true_type isv;
 
   const unsigned dk = st32, dv = st32 + SH::TILE;
-  const char* const kbuf = st;
   const char* const vbuf = st + SH::TILE;
+  const unsigned rb = row_base<D>(lane), cb = col_base<D>(lane);
   unsigned ok = 0;
   if (nt > 0) {
     ok = issue(isk, ka, dk);
@@ -297,8 +326,7 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
     for (int t = 0; t < RT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const s16x8 a0 = fa::ld_row8<D, false>(kbuf, c16, k, g);
-      const s16x8 a1 = fa::ld_row8<D, false>(kbuf, 16 + c16, k, g);
+      const s16x8 a0 = read_row<D>(dk, rb, 0, k), a1 = read_row<D>(dk, rb, 1, k);
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         s[t][0] = fa::Mfma<T>::run(a0, qf[t][k], s[t][0]);
@@ -315,7 +343,7 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 16 * h + 4 * g + e;
-            if (!((here >> r) & 1) || kt + r >= lim[t]) s[t][h][e] = -INFINITY;
+            if (!((here >> (4 * g)) & (1u << (16 * h + e))) || kt + r >= lim[t]) s[t][h][e] = -INFINITY;
           }
     }
     // The base moves only when a score outgrows it by 2^8; whether one does needs no look at other lanes.
@@ -380,7 +408,7 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
         constexpr short ONE = __is_same(T, f16_t) ? 0x3c00 : 0x3f80, INF = __is_same(T, f16_t) ? 0x7c00 : 0x7f80;
 #pragma unroll 1
         for (int d = 0; d < DB; ++d) {
-          const s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+          const s16x8 v = read_col<D>(dv, cb, 0, d);
           unsigned note[RT];
 #pragma unroll
           for (int t = 0; t < RT; ++t) note[t] = 0;
@@ -414,7 +442,7 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
     }
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
-      const s16x8 v = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+      const s16x8 v = read_col<D>(dv, cb, 0, d);
 #pragma unroll
       for (int t = 0; t < RT; ++t) acc[t][d] = fa::Mfma<T>::run(v, pf[t], acc[t][d]);
     }
@@ -488,6 +516,11 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
 // layout of item() each wave reads all of its own keys from L2, 32 rows at a time: at 2048 rows a key head that
 // is 19 TB/s of L2 reads, which bound it (518 TFLOP/s); here a tile serves 8 times as many rows.
 constexpr int kWideRT = 2;
+// Tiles between two meetings of a block's waves: what LDS holds in rings of twice as many
+template <int D>
+constexpr int wide_depth() {
+  return D <= 64 ? 2 : 1;
+}
 
 // Asks the scheduler for N times one matrix instruction, three vector ones and an exponential behind it: the
 // matrix cores run while the wave issues the others
@@ -506,6 +539,7 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
   using SH = Shared<T, D, NW>;
   constexpr int KS = D / 32, DB = D / 16, TILE = 64 * D * 2, ND = 64 / SH::RPI / NW;  // DMA instructions a wave, K or V
   static_assert(ND * SH::RPI * NW == 64, "a tile's rows divide over the waves");
+  constexpr int DEPTH = wide_depth<D>();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
   row0 += wave * 16 * RT;
@@ -536,21 +570,31 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
   const bool grouped = A.page % SH::RPI == 0;
   Window win{A.ptable, A.pblocks, 0, -1};
   if (nt > 0) win.load(page_of(k0));
-  unsigned sk[ND], sv[ND];
+  unsigned sk[ND], sv[ND];  // byte offsets from the first row of an instruction
 #pragma unroll
   for (int i = 0; i < ND; ++i) {
     const int row = (wave * ND + i) * SH::RPI + rl;
-    sk[i] = (unsigned)(cl ^ fa::swz_b128<D>(row)) << 4;
-    sv[i] = (unsigned)(cl ^ fa::swz_tr<D>(row)) << 4;
+    sk[i] = (unsigned)(rl * (int)A.cr * 2) + ((unsigned)(cl ^ fa::swz_b128<D>(row)) << 4);
+    sv[i] = (unsigned)(rl * (int)A.cr * 2) + ((unsigned)(cl ^ fa::swz_tr<D>(row)) << 4);
   }
-  const unsigned rowb = (unsigned)(rl * (int)A.cr * 2);
 
   // Places of a tile's 64 keys: byte offset of key kt + lane from the head's base, and which keys exist
   struct Places {
     unsigned lo, hi;
     unsigned long long ok;
   };
+  const bool aligned = A.page % 64 == 0;  // a tile lies in one page
+  const unsigned lane_off = (unsigned)lane * (unsigned)A.cr * 2;
   auto places = [&](int kt) -> Places {
+    if (aligned) {
+      const int p = page_of(kt);
+      if (p - win.w0 >= 64) win.load(p);
+      const int blk = __builtin_amdgcn_readlane(win.val, p - win.w0);
+      const unsigned long long off =
+          (unsigned long long)((long long)blk * A.cb + (long long)(kt - p * A.page) * A.cr) * 2 + lane_off;
+      return Places{(unsigned)off, (unsigned)(off >> 32),
+                    (unsigned)blk < (unsigned)A.num_blocks ? (unsigned long long)__ballot(kt + lane < k1) : 0ull};
+    }
     const int p1 = page_of(min(kt + 63, k1 - 1));
     if (p1 - win.w0 >= 64) win.load(page_of(kt));  // 64 pages hold a tile
     const int key = kt + lane, pg = min(page_of(key), p1), blk = win.at(pg);
@@ -559,7 +603,8 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
                   (unsigned long long)__ballot(key < k1 && (unsigned)blk < (unsigned)A.num_blocks)};
   };
   // this wave's rows of a tile's K (or V)
-  auto issue = [&](const Places& p, const char* base, const unsigned (&sw)[ND], unsigned dst) {
+  auto issue = [&](auto isv, const Places& p, unsigned dst) {
+    const char* const base = isv ? vh : kh;
     dst += wave * ND * 1024;
     if (p.ok == ~0ull && grouped) {
 #pragma unroll
@@ -567,22 +612,28 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
         const int r = (wave * ND + i) * SH::RPI;
         const unsigned long long o = (unsigned long long)(unsigned)__builtin_amdgcn_readlane(p.lo, r) |
                                      (unsigned long long)(unsigned)__builtin_amdgcn_readlane(p.hi, r) << 32;
-        fa::fa_glds(base + o, rowb + sw[i], dst + i * 1024);
+        fa::fa_glds(base + o, isv ? sv[i] : sk[i], dst + i * 1024);
       }
     } else {
+      int ln = lane;
+      asm volatile("" : "+v"(ln));  // rare: its addresses are formed here, not kept in registers through the loop
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        const int r = (wave * ND + i) * SH::RPI + rl;
+        const int r = (wave * ND + i) * SH::RPI + ln / (D / 8);
+        const unsigned sw = (unsigned)((ln % (D / 8)) ^ (isv ? fa::swz_tr<D>(r) : fa::swz_b128<D>(r))) << 4;
         const unsigned long long o = (unsigned long long)(unsigned)__shfl((int)p.lo, r, 64) |
                                      (unsigned long long)(unsigned)__shfl((int)p.hi, r, 64) << 32;
-        glds64(((p.ok >> r) & 1) ? base + o + sw[i] : reinterpret_cast<const char*>(g_zero_row) + sw[i], dst + i * 1024);
+        glds64(((p.ok >> r) & 1) ? base + o + sw : reinterpret_cast<const char*>(g_zero_row) + sw, dst + i * 1024);
       }
     }
   };
 
+  std::false_type isk;
+  std::true_type isv;
   f32x4 s[RT][4], c[RT][4];
   float mx[RT], over = -INFINITY;
-  auto scores = [&](const char* kbuf, f32x4 (&o)[RT][4]) {
+  const unsigned rb = row_base<D>(lane), cb = col_base<D>(lane);
+  auto scores = [&](unsigned kbuf, f32x4 (&o)[RT][4]) {
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -591,20 +642,22 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const s16x8 a = fa::ld_row8<D, false>(kbuf, 16 * h + c16, k, g);
+        const s16x8 a = read_row<D>(kbuf, rb, h, k);
 #pragma unroll
         for (int t = 0; t < RT; ++t) o[t][h] = fa::Mfma<T>::run(a, qf[t][k], o[t][h]);
       }
   };
   auto mask = [&](unsigned long long ok, f32x4 (&o)[RT][4]) {
     if (ok != ~0ull) {
+      const unsigned long long mine = ok >> (4 * g);  // key 16 h + 4 g + e at bit 16 h + e
+      const unsigned w[2] = {(unsigned)mine, (unsigned)(mine >> 32)};
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int h = 0; h < 4; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!((ok >> (16 * h + 4 * g + e)) & 1)) o[t][h][e] = -INFINITY;
+            if (!(w[h >> 1] & (1u << (16 * (h & 1) + e)))) o[t][h][e] = -INFINITY;
     }
   };
   auto maxima = [&](const f32x4 (&o)[RT][4]) {
@@ -636,110 +689,127 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
     }
   };
 
-  // LDS: two buffers of K, two of V.  Pipeline: while a tile's probabilities are formed, the next tile's scores
-  // are on the matrix cores.
-  Places pl{0, 0, 0};
-  unsigned long long ok = 0;
-  if (nt > 0) {
-    pl = places(k0);
-    ok = pl.ok;
-    issue(pl, kh, sk, st32);
-    issue(pl, vh, sv, st32 + 2 * TILE);
-    if (nt > 1) {
-      pl = places(k0 + 64);
-      issue(pl, kh, sk, st32 + TILE);
-    }
-    wait_vm<0>();
-    __syncthreads();
-    scores(smem, s);
-    mask(ok, s);
-    maxima(s);
-    rebase();
-  }
-  for (int it = 0; it < nt; ++it) {
-    const bool more = it + 1 < nt;
-    wait_vm<0>();
-    __syncthreads();  // V of this tile and K of the next are here, and every wave is done with the ones before
-    if (more) issue(pl, vh, sv, st32 + (2 + ((it + 1) & 1)) * TILE);
-    ok = pl.ok;
-    if (it + 2 < nt) {
-      pl = places(k0 + 64 * (it + 2));
-      issue(pl, kh, sk, st32 + (it & 1) * TILE);
-    }
-    const char* const kbuf = smem + ((it + 1) & 1) * TILE;
-    const char* const vbuf = smem + (2 + (it & 1)) * TILE;
-    // Phase 1: 8 RT / 2 products a step with a part of the probabilities under them, the operands of the next
-    // step on their way from LDS; phase 2: the product with the values, four operands ahead.  The barriers keep
+  // LDS: rings of 2 DEPTH tiles of K and of V.  Pipeline: while a tile's probabilities are formed, the next tile's
+  // scores are on the matrix cores.  The waves meet once in DEPTH tiles, and fetch as many.
+  constexpr int RING = 2 * DEPTH;
+  const unsigned kr = st32, vr = st32 + RING * TILE;
+  auto exists = [&](int t) { return t < nt; };
+  auto tile = [&](int it, auto u, const f32x4 (&s)[RT][4], f32x4 (&c)[RT][4], unsigned long long ok) {
+    const unsigned kbuf = kr + ((DEPTH == 1 ? u + 1 : it + 1) % RING) * TILE;
+    const unsigned vbuf = vr + ((DEPTH == 1 ? u : it) % RING) * TILE;
+    // Phase 1: FG RT products a step with a part of the probabilities under them, the operands of the next step on
+    // their way from LDS; phase 2: the product with the values, likewise a step ahead.  The barriers keep
     // the compiler from sinking each read to its product, where a wave would wait out the LDS's latency 48
     // times a tile.  (Behind the last tile the scores are of stale bytes, and never used.)
-    s16x8 pf[RT][2], fr[2][4];
+    constexpr int FG = D == 256 ? 4 : 2, NK = 4 * KS / FG, NV = 2 * DB / FG;  // operands a step, steps of the phases
+    s16x8 pf[RT][2], fr[2][FG];
+    auto read = [&](int step, s16x8 (&f)[FG]) {  // operand i of phase 1: keys 16 (i % 4), values 32 (i / 4) of K
 #pragma unroll
-    for (int h = 0; h < 4; ++h) fr[0][h] = fa::ld_row8<D, false>(kbuf, 16 * h + c16, 0, g);
+      for (int j = 0; j < FG; ++j) {
+        const int i = step * FG + j, v = i - 4 * KS;
+        f[j] = v < 0 ? read_row<D>(kbuf, rb, i & 3, i >> 2) : read_col<D>(vbuf, cb, v / DB, v % DB);
+      }
+    };
+    read(0, fr[0]);
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int h = 0; h < 4; ++h) c[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      if (k + 1 < KS) {
+    for (int k = 0; k < NK; ++k) {
+      read(k + 1, fr[(k + 1) & 1]);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) fr[(k + 1) & 1][h] = fa::ld_row8<D, false>(kbuf, 16 * h + c16, k + 1, g);
-      } else {
+      for (int j = 0; j < FG; ++j) {
+        const int i = k * FG + j;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) fr[(k + 1) & 1][d] = fa::ld_tr8<D, true>(vbuf, 0, d, lane);
+        for (int t = 0; t < RT; ++t) c[t][i & 3] = fa::Mfma<T>::run(fr[k & 1][j], qf[t][i >> 2], c[t][i & 3]);
       }
 #pragma unroll
-      for (int h = 0; h < 4; ++h)
+      for (int i = 0; i < 4 * RT; ++i)  // part i of the probabilities: row tile i / 4, 16 keys i % 4
+        if (i * NK / (4 * RT) == k) {
+          const int t = i / 4, h = i % 4;
+          float p[4];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) c[t][h] = fa::Mfma<T>::run(fr[k & 1][h], qf[t][k], c[t][h]);
+          for (int e = 0; e < 4; ++e) p[e] = fa::fast_exp2(s[t][h][e] * A.scale + nm[t]);
+          l[t] += (p[0] + p[1]) + (p[2] + p[3]);
+          const unsigned w[2] = {fa::f2s2<T>(p[0], p[1]), fa::f2s2<T>(p[2], p[3])};
+          const s16x4 q = __builtin_bit_cast(s16x4, w);
 #pragma unroll
-      for (int i = 0; i < 2 * RT; ++i)  // part i of the probabilities: row tile i / 2, 32 keys i % 2
-        if (i * KS / (2 * RT) == k) {
-          const int t = i / 2, j = i % 2;
-          float p[2][4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[h][e] = fa::fast_exp2(s[t][2 * j + h][e] * A.scale + nm[t]);
-          l[t] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
-          unsigned w[4];
-          w[0] = fa::f2s2<T>(p[0][0], p[0][1]);
-          w[1] = fa::f2s2<T>(p[0][2], p[0][3]);
-          w[2] = fa::f2s2<T>(p[1][0], p[1][1]);
-          w[3] = fa::f2s2<T>(p[1][2], p[1][3]);
-          pf[t][j] = __builtin_bit_cast(s16x8, w);
+          for (int e = 0; e < 4; ++e) pf[t][h / 2][4 * (h % 2) + e] = q[e];
         }
-      interleave<4 * RT>();
+      interleave<FG * RT>();
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int q = 0; q < 2 * DB / 4; ++q) {  // operands 4 q ..: 32 keys (4 q) / DB, values (4 q) % DB ..
-      if (q + 1 < 2 * DB / 4) {
+    for (int q = 0; q < NV; ++q) {
+      if (q + 1 < NV) read(NK + q + 1, fr[(NK + q + 1) & 1]);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const int i = 4 * (q + 1) + d;
-          fr[(KS + q + 1) & 1][d] = fa::ld_tr8<D, true>(vbuf, 32 * (i / DB), i % DB, lane);
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int i = 4 * q + d;
+      for (int j = 0; j < FG; ++j) {
+        const int i = q * FG + j;  // values 16 (i % DB) of keys 32 (i / DB)
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-          acc[t][i % DB] = fa::Mfma<T>::run(fr[(KS + q) & 1][d], pf[t][i / DB], acc[t][i % DB]);
+          acc[t][i % DB] = fa::Mfma<T>::run(fr[(NK + q) & 1][j], pf[t][i / DB], acc[t][i % DB]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int h = 0; h < 4; ++h) s[t][h] = c[t][h];
-    if (more) {
-      mask(ok, s);
-      maxima(s);
+    if (exists(it + 1)) {
+      mask(ok, c);
+      maxima(c);
       rebase();
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+  Places ahead{0, 0, 0};         // of the last tile whose K was asked for
+  unsigned long long ok1 = 0, next = 0;  // keys of the next tile (DEPTH 2), and of the one after the next two
+  if (nt > 0) {
+    Places pl = places(k0);
+    const unsigned long long ok0 = pl.ok;
+    issue(isk, pl, kr);
+    issue(isv, pl, vr);
+#pragma unroll
+    for (int t = 1; t <= DEPTH; ++t)
+      if (exists(t)) {
+        ahead = places(k0 + 64 * t);
+        if (t == 1) ok1 = ahead.ok;
+        issue(isk, ahead, kr + t * TILE);
+        if (t < DEPTH) issue(isv, ahead, vr + t * TILE);
+      }
+    wait_vm<0>();
+    __syncthreads();
+    scores(kr, s);
+    mask(ok0, s);
+    maxima(s);
+    rebase();
+  }
+  for (int it = 0; it < nt; it += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i = it + u;
+      if (!exists(i)) break;
+      unsigned long long m = ok1;  // keys of tile i + 1
+      if (u % DEPTH == 0) {
+        wait_vm<0>();
+        __syncthreads();  // what was asked for is here, and every wave is done with what it replaces
+        if constexpr (DEPTH == 1) m = ahead.ok;
+        if (exists(i + DEPTH)) issue(isv, ahead, vr + (i + DEPTH) % RING * TILE);
+        if constexpr (DEPTH == 2) ok1 = ahead.ok;
+        if (exists(i + DEPTH + 1)) {
+          ahead = places(k0 + 64 * (i + DEPTH + 1));
+          issue(isk, ahead, kr + (i + DEPTH + 1) % RING * TILE);
+          if constexpr (DEPTH == 2) {
+            issue(isv, ahead, vr + (i + 3) % RING * TILE);
+            next = ahead.ok;
+            if (exists(i + 4)) {
+              ahead = places(k0 + 64 * (i + 4));
+              issue(isk, ahead, kr + (i + 4) % RING * TILE);
+            }
+          }
+        }
+      } else {
+        ok1 = next;
+      }
+      if (u == 0) tile(i, std::integral_constant<int, 0>{}, s, c, m);
+      else tile(i, std::integral_constant<int, 1>{}, c, s, m);
+    }
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
@@ -760,29 +830,19 @@ __device__ __forceinline__ void seq_rows(const Args& A, int b, int& tok0, int& n
   if (tok0 < 0 || n < 0 || tok0 + n > A.T || n > A.most) n = 0;  // offsets that do not fit the call: nothing is read
 }
 
-// Items in the order of dispatch: groups of 8 blocks (one per XCD) of prefix and own items in turn, so that
-// the prefix's products and the own pages' stream share the chip; each XCD has a contiguous part of the
-// items, whose row tiles over the same keys are neighbours and meet in its L2.
+// Items in the order of dispatch, 8 blocks at a time (one per XCD): the prefix items, which take longest, then the
+// own ones.  (Blocks go to the shader engines of an XCD in turn: an alternation of the kinds puts all the long ones
+// on some of them, and the others wait.)  Each XCD has a contiguous part of the items, whose row tiles over the same
+// keys are neighbours and meet in its L2.
 // RTP = 0: wide prefix items (of kWideRT row tiles a wave)
 template <typename T, int D, int RTP, int RTO, int NW>
 __global__ __launch_bounds__(NW * 64) void items_kernel(Args A) {
-  constexpr int RTM = RTP > RTO ? RTP : RTO, narrow = lds_bytes<RTM, D, NW>(), wide = RTP == 0 ? 2 * 2 * 64 * D * 2 : 0;
+  constexpr int RTM = RTP > RTO ? RTP : RTO, narrow = lds_bytes<RTM, D, NW>(), wide = RTP == 0 ? 4 * wide_depth<D>() * 64 * D * 2 : 0;
   __shared__ __attribute__((aligned(16))) char smem[narrow > wide ? narrow : wide];
   const int np = A.Hkv * A.ntp * A.nsp, no = A.B * A.Hkv * A.nto * A.nso;
   const int gp = (np + 7) / 8, go = (no + 7) / 8, x = blockIdx.x & 7;
-  int j = blockIdx.x >> 3;
-  // Two of the prefix, one own, while both last: blocks go to the four shader engines of an XCD in turn, and
-  // an order of period two would leave all the long ones on half of them.
-  const int n3 = min(gp / 2, go);
-  bool prefix;
-  if (j < 3 * n3) {
-    prefix = j % 3 != 2;
-    j = prefix ? j / 3 * 2 + j % 3 : j / 3;
-  } else {
-    j -= 3 * n3;
-    prefix = j < gp - 2 * n3;
-    j = prefix ? j + 2 * n3 : j - (gp - 2 * n3) + n3;
-  }
+  const bool prefix = (int)(blockIdx.x >> 3) < gp;
+  const int j = (int)(blockIdx.x >> 3) - (prefix ? 0 : gp);
   const bool direct = A.wa == nullptr;
   if (prefix) {
     const int id = x * gp + j;
@@ -912,20 +972,27 @@ PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, i
     if (len <= 0) return 0;
     const long long cap = (len + 64 * nw - 1) / (64 * nw);  // two tiles a wave at least
     long long n = (target + items - 1) / items;
-    const long long floor_ = (len + 8191) / 8192;           // no block walks more than 8192 keys alone
-    if (n < floor_) n = floor_;
+    const long long least = (len + 8191) / 8192;            // no block walks more than 8192 keys alone
+    if (n < least) n = least;
     return n < 1 ? 1 : (n > cap ? cap : n);
   };
-  // two blocks a CU of each kind
+  const bool wide = pfx_wide((long long)T * G, D);
   out[0] = (int)ntp;
-  out[1] = (int)ranges(plen, Hkv * ntp, 512);
+  if (wide) {
+    // Beside own keys one round of blocks on 3/4 of the CUs, while the rest stream the own pages (256 sequences
+    // behind 32768 shared keys and 500 .. 1500 of their own: 531 us; 573 with 256 blocks, 599 with 512); alone, two
+    // rounds.  At least 1024 keys a block: 8192 keys in ranges of 512 take 76 us beside 64 sequences, of 1024 70.
+    const long long cap = (plen + 1023) / 1024, n = (own > 0 ? 192 : 512) / (Hkv * ntp);
+    out[1] = plen <= 0 ? 0 : (int)(n < 1 ? 1 : (n > cap ? cap : n));
+  } else {
+    out[1] = (int)ranges(plen, Hkv * ntp, 512);  // two blocks a CU
+  }
   out[2] = (int)nto;
-  long long no = ranges(own, (long long)B * Hkv * nto, 512);
-  out[3] = (int)no;
+  out[3] = (int)ranges(own, (long long)B * Hkv * nto, 512);
   if (out[1] + out[3] == 0) out[3] = 1;
   // one range for every row: written straight to the output; not with packed queries, of which some rows may
   // belong to no sequence and are the join's to clear
-  out[4] = out[1] + out[3] == 1 && !packed && !(out[1] && pfx_wide((long long)T * G, D)) ? 0 : out[1] + out[3];
+  out[4] = out[1] + out[3] == 1 && !packed && !(out[1] && wide) ? 0 : out[1] + out[3];
   return 0;
 }
 

@@ -265,7 +265,12 @@ def attention_case(dev, hq, hkv, d, page, plen, own, new, dtype, seed=0, scale=N
     (6, 2, 64, 16, 40, [12, 40, 3, 9], [5, 33, 3, 0], BF),   # ragged chunks, one sequence without new tokens
     (8, 1, 128, 64, 130, [90, 70], [90, 3], HF),
     (4, 4, 256, 8, 17, [30, 18], [18, 17], BF),
-    (16, 1, 64, 16, 16, [6, 2], [4, 2], BF)])
+    (16, 1, 64, 16, 16, [6, 2], [4, 2], BF),
+    (16, 2, 64, 16, 200, [3, 40] * 20, None, BF),        # prefix items of many rows
+    (8, 1, 128, 64, 333, [5] * 33, None, HF),
+    (8, 1, 128, 5, 203, [5] * 17, None, BF),
+    (16, 1, 256, 8, 130, [2, 33] * 5, None, BF),
+    (12, 2, 128, 32, 1200, [30, 40], [30, 25], BF)])
 def test_attention(dev, hq, hkv, d, page, plen, own, new, dtype):
     attention_case(dev, hq, hkv, d, page, plen, own, new, dtype, behind=0 if new is None else 2)
 
@@ -279,6 +284,8 @@ def test_attention_empty_and_long_parts(dev):
     attention_case(dev, 2, 1, 64, 16, 37, [33, 64], None, BF, scale=0.37, sharp=4.0)   # sharp rows
     attention_case(dev, 2, 1, 128, 16, 64, [2100, 3], None, HF)           # more pages than a wave's window
     attention_case(dev, 2, 1, 64, 1, 150, [170, 3], None, HF)
+    attention_case(dev, 16, 1, 128, 1, 150, [0, 3] * 5, None, BF)
+    attention_case(dev, 32, 2, 64, 16, 4500, [0, 3] * 5, None, BF, device_len=True)
 
 
 @pytest.mark.parametrize('dev', DEVICES)
