@@ -175,13 +175,14 @@ _SIGS = {
                         I, P],
     'pa_prefix_attn_plan': [I, I, I, I, I, I, I, LL, LL, IP],
     'pa_prefix_attn': [P, P, P, LL, LL, LLP, P, LL, I, P, I, P, I, I, I, P, P, P, P, P, P, IP, I, I, I, I, I, I, F, I, P],
-    'pa_sample': [P, LL, I, I, P, I, P, P, P, P, D, I, D, D, P, P, I, P],
+    'pa_sample_ws_bytes': [I],
+    'pa_sample': [P, LL, I, I, P, I, P, P, P, P, D, I, D, D, P, P, P, I, P],
     'pa_flash_fwd': [P, P, P, P, P, I, I, I, I, I, I, LLP, LLP, LLP, LLP, F, I, I, P],
     'pa_flash_bwd': [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, LLP, LLP, LLP, LLP, LLP, LLP, LLP, LLP, F, I, I,
                      P],
 }
 
-_LL_RET = {'pa_bn_ws_floats', 'pa_skinny_ws_floats', 'pa_woq_ws_floats', 'pa_flash_ds_ws_elems'}
+_LL_RET = {'pa_sample_ws_bytes', 'pa_bn_ws_floats', 'pa_skinny_ws_floats', 'pa_woq_ws_floats', 'pa_flash_ds_ws_elems'}
 _VOID_RET = {'pa_adamw_tune', 'pa_act_fwd_tune', 'pa_act_cs_tune'}
 
 

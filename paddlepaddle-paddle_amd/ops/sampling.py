@@ -30,7 +30,7 @@ def composite(x, u, temperature, top_k, top_p, min_p):
     w, at = torch.sort(xd, dim=-1, descending=True, stable=True)
     top, token = w[:, :1], w > float('-inf')
     w = torch.exp((w - top) / torch.where(greedy, torch.ones_like(t), t))
-    w = torch.where(torch.isnan(w) | (torch.isinf(top) & (xd.gather(1, at) == top)), torch.ones_like(w), w)
+    w = torch.where(torch.isinf(top), (xd.gather(1, at) == top).double(), w)  # +inf beside anything finite
     col = torch.arange(V, device=x.device)[None]
     w = torch.where(token & (col < torch.where(greedy, torch.ones_like(k), torch.where(k > 0, k, V))), w, 0.0)
     kept = (w.cumsum(-1) - w < p * w.sum(-1, keepdim=True)) | (p >= 1) | (col == 0)
@@ -63,8 +63,12 @@ def sample(x, u, temperature, top_k, top_p, min_p):
                                               setting(top_p, torch.float32), setting(min_p, torch.float32))
     ids = torch.empty(rows, 1, dtype=torch.int64, device=x.device)
     probs = torch.empty(rows, 1, dtype=torch.float32, device=x.device)
+    if rows == 0:
+        return probs, ids
+    # this call's own workspace: two streams or two captured graphs never share one
+    ws = torch.empty(rows * N.lib.pa_sample_ws_bytes(V), dtype=torch.uint8, device=x.device)
     with N.device_of(x):
         N.check(N.lib.pa_sample(N.ptr(x), x.stride(0), rows, V, N.ptr(u), int(u.dtype == torch.float64), tp, kp, pp, mp,
-                                float(t0), int(k0), float(p0), float(m0), N.ptr(ids), N.ptr(probs), N.dtcode(x.dtype),
+                                float(t0), int(k0), float(p0), float(m0), N.ptr(ids), N.ptr(probs), N.ptr(ws), N.dtcode(x.dtype),
                                 N.stream()), 'sample')
     return probs, ids

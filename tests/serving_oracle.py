@@ -95,7 +95,7 @@ def sample(x, u, t, k, p, m):
     if not t > 0:
         return order[0], 1.0
     top = x[order[0]]
-    w = {i: 1.0 if x[i] == top else math.exp((x[i] - top) / t) for i in order}
+    w = {i: 1.0 if x[i] == top else (0.0 if top == math.inf else math.exp((x[i] - top) / t)) for i in order}
     if k > 0:
         order = order[:k]
     if p < 1:

@@ -466,6 +466,29 @@ def test_sampling_ties_and_masks(dev):
 
 
 @pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('vocab,dtype', [(8192, FF), (8193, BF), (20001, FF), (40000, HF)])
+def test_sampling_large_vocabularies(dev, vocab, dtype):
+    """Several chunks; borders in bins of few tokens, and of more than the kernel ranks (flat rows, many ties)."""
+    g = torch.Generator().manual_seed(vocab)
+    rows = 8
+    x = torch.randn(rows, vocab, generator=g) * 2.5
+    x[:, ::997] += 6.0
+    x[1] = 0.25                                                         # one value
+    x[2] = torch.randint(0, 2, (vocab,), generator=g).float()           # two values
+    x[3, vocab // 2:] = float('-inf')
+    x[4] *= 0.01                                                        # nearly flat
+    x[5], x[5, vocab - 1] = float('-inf'), 1.0                          # the last token alone
+    x[6] -= 1e4
+    x[7, 17] = float('inf')
+    x = x.to(dtype)
+    u = torch.rand(rows, generator=g, dtype=torch.float64)
+    for t, k, p, m in ((1.0, 0, 1.0, 0.0), (0.7, 0, 0.9, 0.0), (1.0, vocab // 3, 1.0, 0.0), (1.0, vocab // 3, 0.7, 0.0),
+                       (0.8, 50, 0.95, 0.02), (1.0, 0, 1.0, 0.9), (3.0, 0, 0.999, 1e-3), (0.01, 5000, 0.999, 0.0),
+                       (0.0, 0, 1.0, 0.0), (1e-40, 0, 1.0, 0.0), (float('inf'), 0, 0.5, 0.0)):
+        sampling_case(dev, x, u, t, k, p, m)
+
+
+@pytest.mark.parametrize('dev', DEVICES)
 def test_sampling_strided_rows_and_empty(dev):
     g = torch.Generator().manual_seed(9)
     wide = torch.randn(5, 1300, generator=g)
