@@ -22,7 +22,8 @@
 namespace pa {
 namespace smp {
 
-constexpr int NT = 1024;
+constexpr int NT = 512;       // threads of a row's block
+constexpr int NW = NT / 64;
 
 struct Args {
   const void* x;
@@ -111,15 +112,15 @@ constexpr double kLog2e = 1.44269504088896340736;
 
 // A row by radix selection over keys, 8 bits a pass: thresholds by counts (k) and by masses (p).
 template <typename T>
-__device__ void radix_row(const Args& A, int r, uint32_t mk, uint32_t valid, const Setting& c_) {
+__device__ __attribute__((noinline)) void radix_row(const Args& A, int r, uint32_t mk, uint32_t valid, const Setting& c_) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* __restrict__ x = reinterpret_cast<const T*>(A.x) + (long long)r * A.row;
   const int V = A.V, k = c_.k;
   const double p = c_.p, m = c_.m, u = c_.u;
-  __shared__ uint32_t red[16];
+  __shared__ uint32_t red[NW];
   __shared__ uint32_t hist[256];
   __shared__ unsigned long long mass[256];
-  __shared__ double dred[16];
+  __shared__ double dred[NW];
   __shared__ uint32_t sk_, sc_;
   __shared__ unsigned long long sm_;
   const Weigh weigh{(double)value_of(mk), kLog2e / c_.t};
@@ -214,7 +215,7 @@ __device__ void radix_row(const Args& A, int r, uint32_t mk, uint32_t valid, con
   }
 
   // each wave's part of the row: kept mass above the threshold, and its ties
-  const int span = ((V + 15) / 16 + 63) / 64 * 64, a0 = min(wave * span, V), a1 = min(a0 + span, V);
+  const int span = ((V + NW - 1) / NW + 63) / 64 * 64, a0 = min(wave * span, V), a1 = min(a0 + span, V);
   const double wt = weight(tk);
   const bool tie_ok = wt >= m;
   double s = 0.0;
@@ -235,7 +236,7 @@ __device__ void radix_row(const Args& A, int r, uint32_t mk, uint32_t valid, con
   // with the waves before it, each wave's place in the kept mass
   double total = 0.0, before = 0.0;
   uint32_t seen = 0, seen_here = 0;
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < NW; ++i) {
     if (i == wave) { before = total; seen_here = seen; }
     const uint32_t left = ck > seen ? ck - seen : 0, take = red[i] < left ? red[i] : left;
     total += dred[i] + (tie_ok ? take * wt : 0.0);  // one expression for all borders: they meet exactly
@@ -247,7 +248,7 @@ __device__ void radix_row(const Args& A, int r, uint32_t mk, uint32_t valid, con
   int lastw = 0;
   {
     uint32_t sn = 0;
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < NW; ++i) {
       const uint32_t lf = ck > sn ? ck - sn : 0;
       if (dred[i] > 0.0 || (tie_ok && red[i] && lf)) lastw = i;
       sn += red[i];
@@ -297,7 +298,8 @@ __device__ void radix_row(const Args& A, int r, uint32_t mk, uint32_t valid, con
 
 constexpr int CH = 8192;  // tokens of a chunk
 constexpr int NB = 384;   // bins of 1/8 in log2 w: 47.9 octaves, and the last for what lies below
-constexpr int CAP = NT;   // tokens of a border's bin that are ranked
+constexpr int CAP = 1024; // tokens of a border's bin that are listed
+constexpr int MC = 64;    // chunks whose scales are held at a time
 
 struct Chunk {
   uint32_t key, valid, first, pad;  // largest key, tokens, lowest index of the largest
@@ -305,6 +307,14 @@ struct Chunk {
   unsigned long long mass[NB];      // relative to the chunk's largest logit, scaled by kFix
 };
 constexpr double kFix = 562949953421312.0;  // 2^49: 8192 tokens stay under 2^62
+// w kFix rounded to an integer, for w in [0, 1]: added to 2^52, whose last place is 1
+__device__ __forceinline__ unsigned long long fixed(double w) {
+  return __builtin_bit_cast(unsigned long long, fma(w, kFix, 4503599627370496.0)) & 0xfffffffffffffull;
+}
+// a token's place in the order: larger ones come first
+__device__ __forceinline__ unsigned long long place(uint32_t key, uint32_t i) {
+  return (unsigned long long)key << 32 | (0xffffffffu - i);
+}
 
 __device__ __forceinline__ double grid_of(float x, double s) { return floor((double)x * s * 8.0); }
 // Bin of a logit under the largest one's place on the grid.  +inf: bin 0, and the last for what lies under it.
@@ -399,15 +409,20 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
   if (valid == 0 || !(t > 0.0)) return;  // no histogram is read
   const Weigh weigh{(double)value_of(mk), kLog2e / t};
   const double top = grid_of(value_of(mk), weigh.s);
-#pragma unroll
-  for (int j = 0; j < P; ++j)
+  // Rolled, the tokens read again from the caches: at one block a CU the code's own way into the instruction cache is
+  // what takes longest
+#pragma unroll 1
+  for (int j = 0; j < P; ++j) {
+    float q[E];
+    load_tokens<T, E>(x, i0 + (j * 256 + tid) * E, end, vec, q);
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (key_of(v[j][e]) != 0) {
-        const int b = bin_of(v[j][e], weigh.s, top);
+      if (key_of(q[e]) != 0) {
+        const int b = bin_of(q[e], weigh.s, top);
         atomicAdd(&count[b], 1u);
-        if (b < NB - 1) atomicAdd(&mass[b], (unsigned long long)(weigh(v[j][e]) * kFix + 0.5));
+        if (b < NB - 1) atomicAdd(&mass[b], fixed(weigh(q[e])));
       }
+  }
   __syncthreads();
   for (int i = tid; i < NB; i += 256) {
     C->count[i] = count[i];
@@ -430,19 +445,23 @@ __device__ __forceinline__ V wave_scan(V v) {
 // Bounded by latency: some ten dependent steps over a few KB, one re-read of the chunks that have a border's
 // tokens, and one chunk's scan.
 template <typename T>
-__global__ __launch_bounds__(NT) void row_kernel(Args A, const Chunk* __restrict__ in, int nc) {
+__global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restrict__ in, int nc) {
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* __restrict__ x = reinterpret_cast<const T*>(A.x) + (long long)r * A.row;
   const Chunk* const C = in + (long long)r * nc;
-  __shared__ uint32_t rk[16], rv[16], ri[16];
-  __shared__ uint32_t cum[NB];              // tokens up to and with a bin
-  __shared__ double cmass[NB];              // and their mass
-  __shared__ uint32_t lkey[CAP], lidx[CAP]; // tokens of a border's bin
-  __shared__ unsigned long long lw[CAP];
-  __shared__ uint32_t ln;
-  __shared__ uint32_t tkey, tidx;           // the last kept token by top-k and top-p
-  __shared__ double dsh, red[16];
-  __shared__ int bsh;
+  struct Token {
+    unsigned long long place, w;              // w: fixed(), 0 once it is not kept
+  };
+  __shared__ uint32_t rk[NW], rv[NW], ri[NW];
+  __shared__ uint32_t cum[NB];                // tokens up to and with a bin
+  __shared__ double cmass[NB];                // and their mass
+  __shared__ Token list[CAP];                 // tokens of a border's bin
+  __shared__ uint32_t ln;                     // their number
+  __shared__ uint32_t pcount[256];
+  __shared__ unsigned long long pmass[256], fsh;
+  __shared__ double red[NW], scale[MC];
+  __shared__ int bsh, shift[MC], with[MC], wn;
+  __shared__ unsigned long long wmax[NW], wmin[NW];
 
   uint32_t mk = 0, mi = 0xffffffffu, valid = 0;
   for (int c = tid; c < nc; c += NT) {
@@ -470,42 +489,56 @@ __global__ __launch_bounds__(NT) void row_kernel(Args A, const Chunk* __restrict
   __syncthreads();
   valid = 0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < NW; ++w) {
     valid += rv[w];
     if (rk[w] > mk || (rk[w] == mk && ri[w] < mi)) {
       mk = rk[w];
       mi = ri[w];
     }
   }
-  const Setting c_ = setting(A, r);
-  if (valid == 0 || !(c_.t > 0.0)) {  // nothing to draw from, or the largest
+  const Setting S = setting(A, r);
+  if (valid == 0 || !(S.t > 0.0)) {  // nothing to draw from, or the largest
     if (tid == 0) {
       A.ids[r] = valid == 0 ? -1 : (int64_t)mi;
       A.probs[r] = valid == 0 ? 0.f : 1.f;
     }
     return;
   }
-  const Weigh weigh{(double)value_of(mk), kLog2e / c_.t};
+  const Weigh weigh{(double)value_of(mk), kLog2e / S.t};
   const double top = grid_of(value_of(mk), weigh.s);
-  // a chunk's scale beside the row, and its bins' shift
-  auto scale_of = [&](int c) -> double { return C[c].key ? weigh(value_of(C[c].key)) * (1.0 / kFix) : 0.0; };
-  auto shift_of = [&](int c) -> int { return C[c].key ? bin_of(value_of(C[c].key), weigh.s, top) : NB; };
-  auto fixed = [](double w) -> unsigned long long { return (unsigned long long)(w * kFix + 0.5); };
+  // the scales of chunks [c0, c0 + MC) beside the row, and their bins' shifts
+  auto scales = [&](int c0) {
+    __syncthreads();
+    if (tid < MC && c0 + tid < nc) {
+      const uint32_t k = C[c0 + tid].key;
+      scale[tid] = k ? weigh(value_of(k)) * (1.0 / kFix) : 0.0;
+      shift[tid] = k ? bin_of(value_of(k), weigh.s, top) : NB;
+    }
+    __syncthreads();
+  };
 
-  // the chunks' histograms, joined; the last bin has what is left of the tokens, and no mass
-  if (tid < NB) {
+  // the chunks' histograms, joined; the last bin has no mass
+  {
     uint32_t n = 0;
     double w = 0.0;
-    if (tid < NB - 1)
-      for (int c = 0; c < nc; ++c) {
-        const int b = tid - shift_of(c);
-        if (b >= 0) {
-          n += C[c].count[b];
-          w += (double)C[c].mass[b] * scale_of(c);
+    for (int c0 = 0; c0 < nc; c0 += MC) {
+      scales(c0);
+      if (tid < NB - 1) {
+        const int e = min(MC, nc - c0);
+#pragma unroll 8
+        for (int c = 0; c < e; ++c) {
+          const int b = tid - shift[c], at = max(b, 0);
+          const uint32_t cn = C[c0 + c].count[at];
+          const double cw = (double)C[c0 + c].mass[at] * scale[c];
+          n += b >= 0 ? cn : 0u;
+          w += b >= 0 ? cw : 0.0;
         }
       }
-    cum[tid] = n;
-    cmass[tid] = w;
+    }
+    if (tid < NB) {
+      cum[tid] = n;
+      cmass[tid] = w;
+    }
   }
   __syncthreads();
   if (wave == 0) {
@@ -527,181 +560,302 @@ __global__ __launch_bounds__(NT) void row_kernel(Args A, const Chunk* __restrict
   }
   __syncthreads();
 
-  // Tokens of bin b into the list.  Their number is known; false where it does not fit.
+  // Tokens of bins [b0, b1], b0 being 0 or b1, into the list.  Their number is known; false where it does not fit.
   const bool vec = vector_rows<T>(A);
   int listed = -1;
-  auto gather = [&](int b) -> bool {
-    if (b == listed) return true;
-    const uint32_t want = cum[b] - (b ? cum[b - 1] : 0u);
-    if (want > CAP) return false;
-    listed = b;
+  auto gather = [&](int b0, int b1) -> bool {
+    if (b1 == listed) return true;
+    if (cum[b1] - (b0 ? cum[b0 - 1] : 0u) > CAP) return false;
+    listed = b1;
     __syncthreads();  // the list before has been read
     if (tid == 0) ln = 0;
-    __syncthreads();
-    for (int c = 0; c < nc; ++c) {
-      const int lb = b - shift_of(c);
-      if (lb < 0 || C[c].count[lb] == 0) continue;
-      float v[8];
-      load_tokens<T, 8>(x, c * CH + tid * 8, min(A.V, (c + 1) * CH), vec, v);
+    for (int c0 = 0; c0 < nc; c0 += MC) {
+      if (nc > MC) scales(c0);
+      if (tid == 0) wn = 0;
+      __syncthreads();
+      if (tid < MC && c0 + tid < nc) {
+        // a chunk's largest token is in its bin 0
+        const int b = b1 - shift[tid];
+        if (b >= 0 && (b0 < b1 || C[c0 + tid].count[b] != 0)) with[atomicAdd(&wn, 1)] = c0 + tid;
+      }
+      __syncthreads();
+      const int n = wn;
+#pragma unroll 1
+      for (int j = 0; j < n * (CH / (8 * NT)); ++j) {  // 8 tokens a thread at a time
+        const int c = with[j / (CH / (8 * NT))], i = c * CH + (j % (CH / (8 * NT)) * NT + tid) * 8;
+        float v[8];
+        load_tokens<T, 8>(x, i, min(A.V, (c + 1) * CH), vec, v);
+        uint32_t hit = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (key_of(v[e]) != 0 && bin_of(v[e], weigh.s, top) == b) {
-          const uint32_t at = atomicAdd(&ln, 1u);
-          if (at < CAP) {
-            lkey[at] = key_of(v[e]);
-            lidx[at] = c * CH + tid * 8 + e;
-            lw[at] = fixed(weigh(v[e]));
-          }
+        for (int e = 0; e < 8; ++e) {
+          const int b = bin_of(v[e], weigh.s, top);
+          if (b >= b0 && b <= b1 && key_of(v[e]) != 0) hit |= 1u << e;
         }
+        while (hit) {
+          const int e = __builtin_ctz(hit);
+          hit &= hit - 1;
+          const float q = to_f(x[i + e]);
+          const uint32_t at = atomicAdd(&ln, 1u);
+          if (at < CAP) list[at] = Token{place(key_of(q), i + e), fixed(weigh(q))};
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
     return true;
   };
-  // of the list: tokens before this one in the order, and their mass (threads below ln)
-  auto rank = [&](uint32_t& before, unsigned long long& mass) {
+  // Of the listed tokens that are kept, in the order of falling places (or rising indexes, BY_INDEX): by count, the one
+  // with `last` before it; by mass, the last one before which less than `room` lies.  `at`: its place; `mass`: up to and
+  // with it.  The range of the order that holds it is cut into 256 parts until few tokens are left to be ranked.
+  constexpr int PER = CAP / NT;
+  auto select = [&](bool by_index, bool by_mass, uint32_t last, unsigned long long room, unsigned long long& at,
+                    unsigned long long& mass) {
     const uint32_t n = ln;
-    before = 0;
-    mass = 0;
-    if ((uint32_t)tid < n) {
-      const uint32_t k = lkey[tid], i = lidx[tid];
-      for (uint32_t j = 0; j < n; ++j)
-        if (lkey[j] > k || (lkey[j] == k && lidx[j] < i)) {
+    Token t[PER];
+    unsigned long long o[PER], hi = 0, lo = ~0ull;  // 0: none
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const uint32_t i = tid + e * NT;
+      t[e] = i < n ? list[i] : Token{0, 0};
+      o[e] = i < n && t[e].w ? (by_index ? t[e].place & 0xffffffffull : t[e].place) : 0;
+      if (o[e]) {
+        hi = max(hi, o[e]);
+        lo = min(lo, o[e]);
+      }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+      hi = max(hi, __shfl_xor(hi, d, 64));
+      lo = min(lo, __shfl_xor(lo, d, 64));
+    }
+    __syncthreads();  // what was before has been read
+    if (lane == 0) {
+      wmax[wave] = hi;
+      wmin[wave] = lo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      hi = max(hi, wmax[w]);
+      lo = min(lo, wmin[w]);
+    }
+    uint32_t n0 = 0, in = n;      // tokens and mass before the window, tokens in it
+    unsigned long long w0 = 0, width = hi - lo;
+    while (in > 32 && width > 0) {
+      const int sh = max(0, 64 - __builtin_clzll(width) - 8);
+      if (tid < 256) {
+        pcount[tid] = 0;
+        pmass[tid] = 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (o[e] && o[e] <= hi && hi - o[e] <= width) {
+          const int q = (int)((hi - o[e]) >> sh);
+          atomicAdd(&pcount[q], 1u);
+          atomicAdd(&pmass[q], t[e].w);
+        }
+      __syncthreads();
+      if (wave == 0) {
+        uint32_t c[4], cs = 0;
+        unsigned long long m[4], ms = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          c[j] = cs += pcount[4 * lane + j];
+          m[j] = ms += pmass[4 * lane + j];
+        }
+        const uint32_t cb = wave_scan(cs) - cs, all = __shfl(cb + cs, 63, 64);
+        const unsigned long long mb = wave_scan(ms) - ms;
+        int best = 255;
+#pragma unroll
+        for (int j = 3; j >= 0; --j) {
+          // (or the last part with a token, where none reaches the mass)
+          const bool here = (by_mass ? w0 + mb + m[j] >= room : n0 + cb + c[j] > last) || cb + c[j] == all;
+          if (here) best = 4 * lane + j;
+          pcount[4 * lane + j] = cb + c[j];
+          pmass[4 * lane + j] = mb + m[j];
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
+        if (lane == 0) bsh = best;
+      }
+      __syncthreads();
+      const int q = bsh;
+      const uint32_t cq = q ? pcount[q - 1] : 0u;
+      in = pcount[q] - cq;
+      n0 += cq;
+      w0 += q ? pmass[q - 1] : 0ull;
+      hi -= (unsigned long long)q << sh;
+      width = min(width - ((unsigned long long)q << sh), (1ull << sh) - 1);
+      __syncthreads();
+    }
+    // the window's tokens, at most 32 of them (one, where its width is 0)
+    if (tid == 0) pcount[0] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (o[e] && o[e] <= hi && hi - o[e] <= width) {
+        const uint32_t i = atomicAdd(&pcount[0], 1u);
+        pmass[i] = o[e];
+        pmass[64 + i] = t[e].w;
+        pmass[128 + i] = t[e].place;
+      }
+    __syncthreads();
+    const uint32_t np = pcount[0];
+    unsigned long long best = 0, bp = 0, bm = 0;  // every thread looks them through: few, and one answer for all
+    if (wave == 0) {
+      const unsigned long long mine = lane < np ? pmass[lane] : 0, w = lane < np ? pmass[64 + lane] : 0;
+      uint32_t before = n0;
+      unsigned long long m = w0;
+      for (uint32_t j = 0; j < np; ++j)
+        if (pmass[j] > mine) {
           ++before;
-          mass += lw[j];
+          m += pmass[64 + j];
         }
+      const bool ok = lane < np && (by_mass ? m < room || before == 0 : before <= last);
+      best = ok ? ~mine : 0;  // the last of them: the smallest
+      bp = ok ? pmass[128 + lane] : 0;
+      bm = ok ? m + w : 0;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) {
+        const unsigned long long b2 = __shfl_xor(best, d, 64), p2 = __shfl_xor(bp, d, 64), m2 = __shfl_xor(bm, d, 64);
+        if (b2 > best) {
+          best = b2;
+          bp = p2;
+          bm = m2;
+        }
+      }
+      if (lane == 0) {
+        wmax[0] = bp;
+        wmin[0] = bm;
+      }
     }
+    __syncthreads();
+    at = wmax[0];
+    mass = wmin[0];
   };
-
-  // top-k: its last token, if it lies in a bin with mass, and the set's mass
-  int bt = NB - 1;        // bin of the last kept token by top-k and top-p; NB - 1: no token with mass is cut
-  bool ok = true;
-  if (tid == 0) {
-    tkey = 0;
-    tidx = 0xffffffffu;
-    dsh = cmass[NB - 1];
-  }
-  __syncthreads();
-  if (c_.k > 0 && (uint32_t)c_.k < valid) {
-    if (tid < NB - 1 && cum[tid] >= (uint32_t)c_.k && (tid == 0 || cum[tid - 1] < (uint32_t)c_.k)) rk[0] = tid;
-    else if (tid == NB - 1 && cum[NB - 2] < (uint32_t)c_.k) rk[0] = NB - 1;
+  auto whole = [](double w) -> unsigned long long { return w > 0.0 ? (unsigned long long)__builtin_ceil(w) : 0ull; };
+  const double ym = (double)value_of(mk) * weigh.s + log2(S.m);  // min-p's border
+  // first bin whose tokens take the mass to the goal
+  auto bin_at = [&](double goal) -> int {
     __syncthreads();
-    bt = (int)rk[0];
-    if (bt < NB - 1) {
-      ok = gather(bt);
-      if (ok) {
-        uint32_t before;
-        unsigned long long mass;
-        rank(before, mass);
-        const uint32_t last = (uint32_t)c_.k - (bt ? cum[bt - 1] : 0u) - 1;  // its rank in the bin
-        if ((uint32_t)tid < ln && before == last) {
-          tkey = lkey[tid];
-          tidx = lidx[tid];
-          dsh = (bt ? cmass[bt - 1] : 0.0) + (double)(mass + lw[tid]) * (1.0 / kFix);
-        }
-      }
-    }
+    if (tid == 0) bsh = NB - 1;
     __syncthreads();
+    if (tid < NB && cmass[tid] >= goal && (tid == 0 || cmass[tid - 1] < goal)) bsh = tid;
+    __syncthreads();
+    return bsh;
+  };
+  const bool topk = S.k > 0 && (uint32_t)S.k < valid && (uint32_t)S.k <= cum[NB - 2];
+  int bk = NB - 1, bm = NB - 1;  // bins of the borders by the histogram
+  if (topk) {
+    if (tid < NB - 1 && cum[tid] >= (uint32_t)S.k && (tid == 0 || cum[tid - 1] < (uint32_t)S.k)) bsh = tid;
+    __syncthreads();
+    bk = bsh;
   }
-  // top-p within it
-  if (ok && c_.p < 1.0) {
-    if (!(c_.p > 0.0)) {  // the first token alone
-      if (tid == 0) {
-        tkey = mk;
-        tidx = mi;
-      }
-      bt = 0;
-      __syncthreads();
-    } else {
-      const double goal = c_.p * dsh;
-      const int bk = bt;
-      if (tid == 0) bsh = NB - 1;
-      __syncthreads();
-      // the first bin whose tokens take the mass to the goal; at or behind top-k's own: that one
-      if (tid < NB && cmass[tid] >= goal && (tid == 0 || cmass[tid - 1] < goal)) bsh = tid;
-      __syncthreads();
-      const int bp = min(bsh, bk);
-      if (bp < NB - 1) {
-        ok = gather(bp);
-        if (ok) {
-          uint32_t before;
-          unsigned long long mass;
-          rank(before, mass);
-          const double above = bp ? cmass[bp - 1] : 0.0;
-          // kept: less than the goal lies before it, and top-k has it
-          const bool in = (uint32_t)tid < ln && (lkey[tid] > tkey || (lkey[tid] == tkey && lidx[tid] <= tidx));
-          const bool kept = in && (above + (double)mass * (1.0 / kFix) < goal || (bp == 0 && before == 0));
-          // the last of them: the one with the most before it
-          uint32_t best = kept ? before + 1 : 0;
-#pragma unroll
-          for (int o = 32; o > 0; o >>= 1) best = max(best, (uint32_t)__shfl_xor(best, o, 64));
-          if (lane == 0) rk[wave] = best;
-          __syncthreads();
-          best = 0;
-#pragma unroll
-          for (int w = 0; w < 16; ++w) best = max(best, rk[w]);
-          // (rounding: none of this bin's, then all of the bins above, whose last token is not looked for)
-          if (best == 0) {
-            if (tid == 0) {
-              tkey = 0xffffffffu;
-              tidx = 0;
-            }
-          } else if (kept && before + 1 == best) {
-            tkey = lkey[tid];
-            tidx = lidx[tid];
-          }
-          bt = bp;
-          __syncthreads();
-        }
-      }
-    }
+  if (S.m > 0.0) {
+    const double d = top - floor(ym * 8.0);
+    bm = d < (double)(NB - 1) ? max((int)d, 0) : (d != d ? 0 : NB - 1);
   }
-  if (!ok) {
-    radix_row<T>(A, r, mk, valid, c_);
-    return;
-  }
-  // min-p: the bin of its border
-  int bf = bt;
-  if (c_.m > 0.0) {
-    const double ym = (double)value_of(mk) * weigh.s + log2(c_.m), d = top - floor(ym * 8.0);
-    const int bm = d < (double)(NB - 1) ? max((int)d, 0) : (d != d ? 0 : NB - 1);
-    if (bm < bf) bf = bm;
-  }
-  // bins before bf are kept whole, of bf what passes the tests, nothing behind it
-  const uint32_t tk = tkey, ti = tidx;
-  auto passes = [&](uint32_t k, uint32_t i, double w) { return (k > tk || (k == tk && i <= ti)) && w >= c_.m; };
-  __shared__ unsigned long long fsh;
-  const bool partial = bf < NB - 1;
-  if (partial) {
-    if (!gather(bf)) {
-      radix_row<T>(A, r, mk, valid, c_);
-      return;
-    }
+  auto weight_of = [&](const Token& t) { return weigh(value_of((uint32_t)(t.place >> 32))); };
+  // Drops what min-p or a place cuts off the list; returns the mass that is left
+  auto keep = [&](unsigned long long tp) -> unsigned long long {
+    __syncthreads();
     if (tid == 0) fsh = 0;
     __syncthreads();
     unsigned long long w = 0;
-    if ((uint32_t)tid < ln) w = passes(lkey[tid], lidx[tid], weigh(value_of(lkey[tid]))) ? lw[tid] : 0;
+    for (uint32_t i = tid; i < ln; i += NT) {
+      if (list[i].place < tp || !(weight_of(list[i]) >= S.m)) list[i].w = 0;
+      w += list[i].w;
+    }
     w = wave_add(w);
     if (lane == 0 && w) atomicAdd(&fsh, w);
     __syncthreads();
-  }
-  const double whole = bf > 0 ? cmass[bf - 1] : 0.0, total = whole + (partial ? (double)fsh * (1.0 / kFix) : 0.0);
-  const double goal = c_.u * total;
+    return fsh;
+  };
 
-  // the chunk in which the kept mass passes the goal: one wave sums a chunk's whole bins and its listed tokens
-  double run = 0.0, start = 0.0;
+  // Steps: the end of top-k's set, the end of top-p's, and with few candidates, all of them on the list, the draw;
+  // else on one border's bin at a time.  (One loop: the selection's code is there once.)
+  const bool nucleus = S.p < 1.0 && S.p > 0.0;
+  int bc = bk;  // candidates: up to this bin; top-k's border is in the list where top-p's goal needs its set's mass
+  if (!(topk && nucleus)) bc = min(min(bk, bm), S.p < 1.0 ? (nucleus ? bin_at(S.p * cmass[NB - 1]) : 0) : NB - 1);
+  const bool few = bc < NB - 1 && cum[bc] <= CAP;
+  int bt = bk;                  // bin of the last token that top-k and top-p keep; NB - 1: none with mass is cut
+  unsigned long long tp = 0;    // its place
+  double set = cmass[NB - 1];   // mass of top-k's set
+  bool ok = true;
+  if (S.p <= 0.0) {             // the first token alone
+    bt = 0;
+    tp = place(mk, mi);
+  }
+#pragma unroll 1
+  for (int step = S.p <= 0.0 || !(topk && (!few || bk == bc)) ? 1 : 0; step < 3 && ok; ++step) {
+    unsigned long long q, m, sum = 0, room = 0;
+    uint32_t last = 0;
+    double above = 0.0;
+    int b = bt;
+    if (step == 1) {
+      if (!nucleus) continue;
+      const double goal = S.p * set;
+      if (!few) {
+        b = min(bin_at(goal), bt);
+        if (b == NB - 1) continue;
+        above = b ? cmass[b - 1] : 0.0;
+      }
+      room = whole((goal - above) * kFix);
+    } else if (step == 0) {
+      last = (uint32_t)S.k - 1 - (!few && b ? cum[b - 1] : 0u);
+      above = !few && b ? cmass[b - 1] : 0.0;
+    } else if (!few) {
+      break;
+    }
+    ok = few ? gather(0, bc) : gather(b, b);
+    if (!ok) break;
+    if (step == 2) {
+      sum = keep(tp);
+      room = (unsigned long long)(S.u < 1.0 ? S.u * (double)sum : (double)sum) + 1;
+    }
+    select(step == 2, step > 0, last, room, q, m);
+    if (step == 0) set = above + (double)m * (1.0 / kFix);
+    if (step == 2) {
+      if (tid == 0) {
+        A.ids[r] = (int64_t)(0xffffffffu - (uint32_t)q);
+        A.probs[r] = (float)(weigh(value_of((uint32_t)(q >> 32))) / ((double)sum * (1.0 / kFix)));
+      }
+      return;
+    }
+    if (b < bt || q > tp) tp = q;
+    bt = b;
+  }
+  // bins before bf are kept whole, of bf what passes the tests, nothing behind it
+  const int bf = min(bt, bm);
+  const bool partial = bf < NB - 1;
+  if (ok && partial) ok = gather(bf, bf);
+  if (!ok) {
+    radix_row<T>(A, r, mk, valid, S);
+    return;
+  }
+  auto passes = [&](unsigned long long at, double w) { return at >= tp && w >= S.m; };
+  const double part = partial ? (double)keep(tp) * (1.0 / kFix) : 0.0;
+  const double total = (bf > 0 ? cmass[bf - 1] : 0.0) + part, goal = S.u * total;
+
+  // the chunk in which the kept mass passes the goal: a wave sums a chunk's whole bins and its listed tokens
+  double run = 0.0, start = 0.0, lastrun = 0.0;
   int at = -1, lastc = -1;
-  double lastrun = 0.0;
-  for (int c0 = 0; c0 < nc && at < 0; c0 += 16) {
+  for (int c0 = 0; c0 < nc && at < 0; c0 += NW) {
+    if (nc > MC && c0 % MC == 0) scales(c0);
     const int c = c0 + wave;
     double w = 0.0;
     if (c < nc) {
-      const int hi = min(bf - shift_of(c), NB - 1);
-      for (int b = lane; b < hi; b += 64) w += (double)C[c].mass[b];
-      w *= scale_of(c);
+      const int hi = min(bf - shift[c % MC], NB - 1);
+#pragma unroll
+      for (int j = 0; j < NB / 64; ++j) {
+        const int b = lane + 64 * j;
+        w += b < hi ? (double)C[c].mass[b] : 0.0;
+      }
+      w *= scale[c % MC];
       if (partial) {
         unsigned long long f = 0;
         for (uint32_t j = lane; j < ln; j += 64)
-          if (lidx[j] / CH == (uint32_t)c && passes(lkey[j], lidx[j], weigh(value_of(lkey[j])))) f += lw[j];
+          if ((0xffffffffu - (uint32_t)list[j].place) / CH == (uint32_t)c) f += list[j].w;
         w += (double)f * (1.0 / kFix);
       }
       w = wave_add(w);
@@ -709,7 +863,7 @@ __global__ __launch_bounds__(NT) void row_kernel(Args A, const Chunk* __restrict
     __syncthreads();
     if (lane == 0) red[wave] = w;
     __syncthreads();
-    for (int j = 0; j < 16 && c0 + j < nc; ++j) {
+    for (int j = 0; j < NW && c0 + j < nc; ++j) {
       const double q = red[j];
       if (q > 0.0) {
         lastc = c0 + j;
@@ -727,53 +881,52 @@ __global__ __launch_bounds__(NT) void row_kernel(Args A, const Chunk* __restrict
     at = lastc;
     start = lastrun;
   }
-  // scan of that chunk, 8 tokens a thread
-  float v[8];
-  double w[8], sum = 0.0;
-  load_tokens<T, 8>(x, at * CH + tid * 8, min(A.V, (at + 1) * CH), vec, v);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t k = key_of(v[e]);
-    w[e] = 0.0;
-    if (k != 0) {
-      const int b = bin_of(v[e], weigh.s, top);
-      if (b < bf || (partial && b == bf)) {
-        const double q = weigh(v[e]);
-        if (b < bf || passes(k, at * CH + tid * 8 + e, q)) w[e] = q;
-      }
+  // Scan of that chunk: the waves' parts, then the part in which the goal is passed, 64 tokens at a time
+  const int i0 = at * CH + wave * (CH / NW), i1 = min(A.V, i0 + CH / NW);
+  auto mass_of = [&](int i) -> double {
+    const float q = i < i1 ? to_f(x[i]) : -INFINITY;
+    const uint32_t k = key_of(q);
+    const int b = k != 0 ? bin_of(q, weigh.s, top) : NB;
+    if (!(b < bf || (partial && b == bf))) return 0.0;
+    const double w = weigh(q);
+    return b < bf || passes(place(k, i), w) ? w : 0.0;
+  };
+  double sum = 0.0;
+#pragma unroll 1
+  for (int i = i0 + lane; i < i1; i += 64) sum += mass_of(i);
+  sum = wave_add(sum);
+  __syncthreads();
+  if (lane == 0) red[wave] = sum;
+  __syncthreads();
+  int mine = -1;
+  double from = 0.0, upto = start;
+  for (int j = 0; j < NW; ++j) {
+    const double next = upto + red[j];
+    if (red[j] > 0.0) {  // (rounding: the last part that has any)
+      mine = j;
+      from = upto;
+      if (next > goal) break;
     }
-    sum += w[e];
+    upto = next;
   }
-  const double inc = wave_scan(sum);
-  __syncthreads();
-  if (lane == 63) red[wave] = inc;
-  if (tid == 0) {
-    rk[0] = 0xffffffffu;  // lowest index that passes the goal
-    rv[0] = 0;            // 1 + the last token with mass
-  }
-  __syncthreads();
-  double before = start + inc - sum;
-  for (int j = 0; j < wave; ++j) before += red[j];
-  uint32_t hit = 0xffffffffu, last = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    before += w[e];
-    if (w[e] > 0.0) {
-      last = tid * 8 + e + 1;
-      if (before > goal && hit == 0xffffffffu) hit = tid * 8 + e;
+  if (wave != mine) return;
+  int found = i0;
+  double share = 0.0;
+#pragma unroll 1
+  for (int i = i0; i < i1; i += 64) {
+    const double w = mass_of(i + lane), c = wave_scan(w);
+    const unsigned long long any = __ballot(w > 0.0), hit = __ballot(w > 0.0 && from + c > goal);
+    if (any) {
+      const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);  // (rounding: the last with mass)
+      found = i + l;
+      share = __shfl(w, l, 64);
+      if (hit) break;
     }
+    from += __shfl(c, 63, 64);
   }
-  if (hit != 0xffffffffu) atomicMin(&rk[0], hit);
-  if (last) atomicMax(&rv[0], last);
-  __syncthreads();
-  const uint32_t found = rk[0] != 0xffffffffu ? rk[0] : rv[0] - 1;  // rounding: the last with mass
-  if ((uint32_t)tid == found / 8) {
-    double q = 0.0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if ((uint32_t)e == found % 8) q = w[e];
-    A.ids[r] = (int64_t)at * CH + found;
-    A.probs[r] = (float)(q / total);
+  if (lane == 0) {
+    A.ids[r] = found;
+    A.probs[r] = (float)(share / total);
   }
 }
 
