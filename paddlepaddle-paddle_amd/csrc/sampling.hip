@@ -36,7 +36,7 @@ struct Args {
   const float* p;
   const float* m;
   double t0, p0, m0;
-  int k0;
+  int k0, own;  // own: bits 0 .. 3, whether t, k, p, m are arrays (else they point to memory that may be read)
   int64_t* ids;
   float* probs;
 };
@@ -51,11 +51,58 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __builtin_bit_cast(float, (k >> 31) ? k & 0x7fffffffu : ~k);
 }
 
+// Lane exchanges by DPP (no trip through LDS): the value of another lane, or 0 where there is none
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V from_lane(V v) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
+  } else {
+    struct Two {
+      int a, b;
+    };
+    Two t = __builtin_bit_cast(Two, v);
+    t.a = __builtin_amdgcn_update_dpp(0, t.a, CTRL, ROWS, 0xf, true);
+    t.b = __builtin_amdgcn_update_dpp(0, t.b, CTRL, ROWS, 0xf, true);
+    return __builtin_bit_cast(V, t);
+  }
+}
+template <typename V>
+__device__ __forceinline__ V lane_value(V v, int lane) {  // of a lane that all lanes name
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    struct Two {
+      int a, b;
+    };
+    Two t = __builtin_bit_cast(Two, v);
+    t.a = __builtin_amdgcn_readlane(t.a, lane);
+    t.b = __builtin_amdgcn_readlane(t.b, lane);
+    return __builtin_bit_cast(V, t);
+  }
+}
+// Inclusive sums over the lanes: shifts by 1, 2, 4, 8 within rows of 16, then the rows' ends to the rows behind
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+  v += from_lane<0x111, 0xf>(v);
+  v += from_lane<0x112, 0xf>(v);
+  v += from_lane<0x114, 0xf>(v);
+  v += from_lane<0x118, 0xf>(v);
+  v += from_lane<0x142, 0xa>(v);
+  v += from_lane<0x143, 0xc>(v);
+  return v;
+}
 template <typename V>
 __device__ __forceinline__ V wave_add(V v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  return lane_value(wave_scan(v), 63);
+}
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+  v = max(v, from_lane<0x111, 0xf>(v));
+  v = max(v, from_lane<0x112, 0xf>(v));
+  v = max(v, from_lane<0x114, 0xf>(v));
+  v = max(v, from_lane<0x118, 0xf>(v));
+  v = max(v, from_lane<0x142, 0xa>(v));
+  v = max(v, from_lane<0x143, 0xc>(v));
+  return lane_value(v, 63);
 }
 
 // 2^y for y <= 0 by its Taylor series around the nearest integer, relative error under 10^-14; 0 under 2^-64
@@ -89,7 +136,7 @@ struct Weigh {
 
 // Down to 10^-30 (0 and below: greedy), where log2(e) / t times a 32-bit logit is far from the 64-bit range's end
 __device__ __forceinline__ double temperature(const Args& A, int r) {
-  const double t = A.t ? (double)A.t[r] : A.t0;
+  const double v = (double)A.t[r], t = A.own & 1 ? v : A.t0;
   return t > 0.0 && t < 1e-30 ? 1e-30 : t;
 }
 
@@ -97,15 +144,20 @@ struct Setting {
   double t, p, m, u;
   int k;
 };
+// (all loads at once: a branch for each setting would wait for them one by one)
 __device__ __forceinline__ Setting setting(const Args& A, int r) {
+  const float p = A.p[r], m_ = A.m[r], u32 = reinterpret_cast<const float*>(A.u)[A.u64 ? 2 * r : r],
+              u32b = reinterpret_cast<const float*>(A.u)[A.u64 ? 2 * r + 1 : r];
+  const int k = A.k[r];
   Setting c;
   c.t = temperature(A, r);
-  c.p = A.p ? (double)A.p[r] : A.p0;
-  const double m = A.m ? (double)A.m[r] : A.m0, u = A.u64 ? reinterpret_cast<const double*>(A.u)[r]
-                                                          : (double)reinterpret_cast<const float*>(A.u)[r];
+  c.p = A.own & 4 ? (double)p : A.p0;
+  const double m = A.own & 8 ? (double)m_ : A.m0;
+  const uint64_t w = (uint64_t)__builtin_bit_cast(uint32_t, u32b) << 32 | __builtin_bit_cast(uint32_t, u32);
+  const double u = A.u64 ? __builtin_bit_cast(double, w) : (double)u32;
   c.m = !(m > 0.0) ? 0.0 : (m < 1.0 ? m : 1.0);
   c.u = u >= 0.0 ? u : 0.0;  // 1 and above: the last kept token
-  c.k = A.k ? A.k[r] : A.k0;
+  c.k = A.own & 2 ? k : A.k0;
   return c;
 }
 constexpr double kLog2e = 1.44269504088896340736;
@@ -300,27 +352,67 @@ constexpr int CH = 8192;  // tokens of a chunk
 constexpr int NB = 384;   // bins of 1/8 in log2 w: 47.9 octaves, and the last for what lies below
 constexpr int CAP = 1024; // tokens of a border's bin that are listed
 constexpr int MC = 64;    // chunks whose scales are held at a time
+constexpr int WITH = 1024;  // parts that are looked through at a time
 
+constexpr int SUB = 512;  // tokens of a part of a chunk: a wave's 8 a lane
 struct Chunk {
   uint32_t key, valid, first, pad;  // largest key, tokens, lowest index of the largest
+  uint32_t part[CH / SUB];          // largest key of each part
   uint32_t count[NB];
-  unsigned long long mass[NB];      // relative to the chunk's largest logit, scaled by kFix
+  unsigned long long mass[NB];      // sums of part_mass()
 };
-constexpr double kFix = 562949953421312.0;  // 2^49: 8192 tokens stay under 2^62
-// w kFix rounded to an integer, for w in [0, 1]: added to 2^52, whose last place is 1
+// A logit on the grid of 1/8 in log2 w: 8 log2 w = (place on the grid) + f, 0 <= f <= 1.  Bin: places under the largest
+// logit's.  +inf: bin 0, f 0, and the last bin for what lies under it.
+struct Grid {
+  double s8, top;
+  __device__ __forceinline__ int bin(float x, double& f) const {
+    const double g = floor((double)x * s8), d = top - g;
+    // (written out: the same weight wherever it is computed; NaN, of infinities: 0; places from 2^53 on: any of [0, 1])
+    f = fmin(fmax(fma((double)x, s8, -g), 0.0), 1.0);
+    return d < (double)(NB - 1) ? (int)d : (d != d ? 0 : NB - 1);
+  }
+  __device__ __forceinline__ int bin(float x) const {
+    double f;
+    return bin(x, f);
+  }
+  // weight, with 1 at the top of bin 0
+  __device__ __forceinline__ double weight(float x) const {
+    double f;
+    const int b = bin(x, f);
+    return exp2_64((f - 1.0 - (double)b) * 0.125);
+  }
+};
+__device__ __forceinline__ Grid grid_of(uint32_t key, double t) {
+  Grid g;
+  g.s8 = 8.0 * kLog2e / t;
+  const double x = (double)value_of(key);
+  g.top = x < INFINITY ? floor(x * g.s8) : INFINITY;  // (also where s8 is 0)
+  return g;
+}
+// 2^(f / 8) scaled by 2^48 and rounded, by its Taylor series around the middle (relative error under 10^-15): what a
+// token adds to its bin's mass
+constexpr double kPart = 281474976710656.0;
+__device__ __forceinline__ unsigned long long part_mass(double f) {
+  const double h = (f - 0.5) * 0.0866433975699931636771;  // ln 2 / 8
+  constexpr double c = 1.0442737824274138403 * kPart;     // 2^(1 / 16)
+  double p = c / 5040.0;
+  p = fma(p, h, c / 720.0);
+  p = fma(p, h, c / 120.0);
+  p = fma(p, h, c / 24.0);
+  p = fma(p, h, c / 6.0);
+  p = fma(p, h, c / 2.0);
+  p = fma(p, h, c);
+  p = fma(p, h, c + 4503599627370496.0);  // on 2^52, whose last place is 1
+  return __builtin_bit_cast(unsigned long long, p) & 0xfffffffffffffull;
+}
+// w scaled by 2^49 and rounded, for w in [0, 1]: a listed token's mass
+constexpr double kFix = 562949953421312.0;
 __device__ __forceinline__ unsigned long long fixed(double w) {
   return __builtin_bit_cast(unsigned long long, fma(w, kFix, 4503599627370496.0)) & 0xfffffffffffffull;
 }
 // a token's place in the order: larger ones come first
 __device__ __forceinline__ unsigned long long place(uint32_t key, uint32_t i) {
   return (unsigned long long)key << 32 | (0xffffffffu - i);
-}
-
-__device__ __forceinline__ double grid_of(float x, double s) { return floor((double)x * s * 8.0); }
-// Bin of a logit under the largest one's place on the grid.  +inf: bin 0, and the last for what lies under it.
-__device__ __forceinline__ int bin_of(float x, double s, double top) {
-  const double d = top - grid_of(x, s);
-  return d < (double)(NB - 1) ? (int)d : (d != d ? 0 : NB - 1);
 }
 
 // E consecutive tokens from i on; -inf past the end
@@ -352,63 +444,61 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
   const T* __restrict__ x = reinterpret_cast<const T*>(A.x) + (long long)r * A.row;
   const int i0 = ch * CH, end = min(A.V, i0 + CH);
   Chunk* const C = out + blockIdx.x;
-  __shared__ uint32_t rk[4], rv[4], ri[4];
+  __shared__ uint32_t rk[CH / SUB], rv, ri;
   __shared__ uint32_t count[NB];
   __shared__ unsigned long long mass[NB];
   for (int i = tid; i < NB; i += 256) {
     count[i] = 0;
     mass[i] = 0;
   }
-  constexpr int E = 8, P = CH / (256 * E);  // a thread's tokens: P times E in a row
+  if (tid == 0) {
+    rv = 0;
+    ri = 0xffffffffu;
+  }
+  constexpr int E = 8, P = CH / (256 * E);  // a thread's tokens: P times E in a row, a wave's: P parts
+  static_assert(SUB == 64 * E, "a part is a wave's");
   float v[P][E];
   const bool vec = vector_rows<T>(A);
-  uint32_t mk = 0, mi = 0xffffffffu, valid = 0;
+  uint32_t valid = 0;
 #pragma unroll
   for (int j = 0; j < P; ++j) load_tokens<T, E>(x, i0 + (j * 256 + tid) * E, end, vec, v[j]);
+  __syncthreads();
 #pragma unroll
-  for (int j = 0; j < P; ++j)
+  for (int j = 0; j < P; ++j) {
+    uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const uint32_t k = key_of(v[j][e]);
       valid += k != 0;
-      if (k > mk) {
-        mk = k;
-        mi = i0 + (j * 256 + tid) * E + e;
-      }
+      m = max(m, k);
     }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t k = __shfl_xor(mk, o, 64), i = __shfl_xor(mi, o, 64);
-    if (k > mk || (k == mk && i < mi)) {
-      mk = k;
-      mi = i;
+    m = wave_max_u(m);
+    if (lane == 0) {
+      rk[j * 4 + wave] = m;
+      C->part[j * 4 + wave] = m;
     }
   }
   valid = wave_add(valid);
-  if (lane == 0) {
-    rk[wave] = mk;
-    ri[wave] = mi;
-    rv[wave] = valid;
-  }
+  if (lane == 0) atomicAdd(&rv, valid);
   __syncthreads();
-  valid = 0;
+  valid = rv;
+  const uint32_t mk = wave_max_u(lane < CH / SUB ? rk[lane] : 0u);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    valid += rv[w];
-    if (rk[w] > mk || (rk[w] == mk && ri[w] < mi)) {
-      mk = rk[w];
-      mi = ri[w];
+  for (int j = 0; j < P; ++j)
+    if (rk[j * 4 + wave] == mk && mk != 0) {  // the part has it
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (key_of(v[j][e]) == mk) atomicMin(&ri, (uint32_t)(i0 + (j * 256 + tid) * E + e));
     }
-  }
+  __syncthreads();
   if (tid == 0) {
     C->key = mk;
     C->valid = valid;
-    C->first = mi;
+    C->first = ri;
   }
   const double t = temperature(A, r);
   if (valid == 0 || !(t > 0.0)) return;  // no histogram is read
-  const Weigh weigh{(double)value_of(mk), kLog2e / t};
-  const double top = grid_of(value_of(mk), weigh.s);
+  const Grid G = grid_of(mk, t);
   // Rolled, the tokens read again from the caches: at one block a CU the code's own way into the instruction cache is
   // what takes longest
 #pragma unroll 1
@@ -418,9 +508,10 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (key_of(q[e]) != 0) {
-        const int b = bin_of(q[e], weigh.s, top);
+        double f;
+        const int b = G.bin(q[e], f);
         atomicAdd(&count[b], 1u);
-        if (b < NB - 1) atomicAdd(&mass[b], fixed(weigh(q[e])));
+        atomicAdd(&mass[b], part_mass(f));
       }
   }
   __syncthreads();
@@ -428,18 +519,6 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
     C->count[i] = count[i];
     C->mass[i] = mass[i];
   }
-}
-
-// inclusive sums over the lanes
-template <typename V>
-__device__ __forceinline__ V wave_scan(V v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V b = __shfl_up(v, o, 64);
-    if (lane >= o) v += b;
-  }
-  return v;
 }
 
 // Bounded by latency: some ten dependent steps over a few KB, one re-read of the chunks that have a border's
@@ -459,10 +538,12 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   __shared__ uint32_t ln;                     // their number
   __shared__ uint32_t pcount[256];
   __shared__ unsigned long long pmass[256], fsh;
-  __shared__ double red[NW], scale[MC];
-  __shared__ int bsh, shift[MC], with[MC], wn;
-  __shared__ unsigned long long wmax[NW], wmin[NW];
+  __shared__ double red[NW];
+  __shared__ uint32_t kmax, kmin;             // their keys
+  __shared__ int bsh, shift[MC], with[WITH], wn;
+  __shared__ unsigned long long got[2];
 
+  const Setting S = setting(A, r);
   uint32_t mk = 0, mi = 0xffffffffu, valid = 0;
   for (int c = tid; c < nc; c += NT) {
     const uint32_t k = C[c].key, i = C[c].first;
@@ -472,15 +553,12 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
       mi = i;
     }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t k = __shfl_xor(mk, o, 64), i = __shfl_xor(mi, o, 64);
-    if (k > mk || (k == mk && i < mi)) {
-      mk = k;
-      mi = i;
-    }
-  }
   valid = wave_add(valid);
+  {
+    const uint32_t k = wave_max_u(mk);
+    mi = ~wave_max_u(mk == k ? ~mi : 0u);  // its lowest index
+    mk = k;
+  }
   if (lane == 0) {
     rk[wave] = mk;
     ri[wave] = mi;
@@ -496,7 +574,6 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
       mi = ri[w];
     }
   }
-  const Setting S = setting(A, r);
   if (valid == 0 || !(S.t > 0.0)) {  // nothing to draw from, or the largest
     if (tid == 0) {
       A.ids[r] = valid == 0 ? -1 : (int64_t)mi;
@@ -504,32 +581,32 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     }
     return;
   }
-  const Weigh weigh{(double)value_of(mk), kLog2e / S.t};
-  const double top = grid_of(value_of(mk), weigh.s);
-  // the scales of chunks [c0, c0 + MC) beside the row, and their bins' shifts
-  auto scales = [&](int c0) {
+  const Grid G = grid_of(mk, S.t);
+  const double wmax = G.weight(value_of(mk));
+  // the shifts of the bins of chunks [c0, c0 + MC)
+  auto shifts = [&](int c0) {
     __syncthreads();
     if (tid < MC && c0 + tid < nc) {
       const uint32_t k = C[c0 + tid].key;
-      scale[tid] = k ? weigh(value_of(k)) * (1.0 / kFix) : 0.0;
-      shift[tid] = k ? bin_of(value_of(k), weigh.s, top) : NB;
+      shift[tid] = k ? G.bin(value_of(k)) : NB;
     }
     __syncthreads();
   };
+  const double bin_scale = exp2_64(-0.125 * (double)(tid + 1)) * (1.0 / kPart);  // of bin tid
 
   // the chunks' histograms, joined; the last bin has no mass
   {
     uint32_t n = 0;
     double w = 0.0;
     for (int c0 = 0; c0 < nc; c0 += MC) {
-      scales(c0);
+      shifts(c0);
       if (tid < NB - 1) {
         const int e = min(MC, nc - c0);
 #pragma unroll 8
         for (int c = 0; c < e; ++c) {
           const int b = tid - shift[c], at = max(b, 0);
           const uint32_t cn = C[c0 + c].count[at];
-          const double cw = (double)C[c0 + c].mass[at] * scale[c];
+          const double cw = (double)C[c0 + c].mass[at];
           n += b >= 0 ? cn : 0u;
           w += b >= 0 ? cw : 0.0;
         }
@@ -537,7 +614,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     }
     if (tid < NB) {
       cum[tid] = n;
-      cmass[tid] = w;
+      cmass[tid] = w * bin_scale;
     }
   }
   __syncthreads();
@@ -560,99 +637,106 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   }
   __syncthreads();
 
-  // Tokens of bins [b0, b1], b0 being 0 or b1, into the list.  Their number is known; false where it does not fit.
+  // Tokens of bins [b0, b1] into the list.  Their number is known; false where it does not fit.  The parts of the row
+  // whose largest token lies before b0's end are read, 16 tokens a lane and two parts a wave at a time.
   const bool vec = vector_rows<T>(A);
   int listed = -1;
   auto gather = [&](int b0, int b1) -> bool {
     if (b1 == listed) return true;
     if (cum[b1] - (b0 ? cum[b0 - 1] : 0u) > CAP) return false;
     listed = b1;
+    constexpr int PP = CH / SUB;
     __syncthreads();  // the list before has been read
-    if (tid == 0) ln = 0;
-    for (int c0 = 0; c0 < nc; c0 += MC) {
-      if (nc > MC) scales(c0);
+    if (tid == 0) {
+      ln = 0;
+      kmax = 0;
+      kmin = 0xffffffffu;
+    }
+    for (int p0 = 0; p0 < nc * PP; p0 += WITH) {
       if (tid == 0) wn = 0;
       __syncthreads();
-      if (tid < MC && c0 + tid < nc) {
-        // a chunk's largest token is in its bin 0
-        const int b = b1 - shift[tid];
-        if (b >= 0 && (b0 < b1 || C[c0 + tid].count[b] != 0)) with[atomicAdd(&wn, 1)] = c0 + tid;
+      for (int p = p0 + tid; p < min(p0 + WITH, nc * PP); p += NT) {
+        const uint32_t k = C[p / PP].part[p % PP];
+        if (k != 0 && G.bin(value_of(k)) <= b1) with[atomicAdd(&wn, 1)] = p;
       }
       __syncthreads();
       const int n = wn;
+      auto fetch = [&](int j, float (&v)[8]) {
+        const int i = j < n ? with[j] * SUB : A.V;
+        load_tokens<T, 8>(x, i + lane * 8, j < n ? min(A.V, i + SUB) : 0, vec, v);
+      };
+      float next[8];
+      fetch(wave, next);
 #pragma unroll 1
-      for (int j = 0; j < n * (CH / (8 * NT)); ++j) {  // 8 tokens a thread at a time
-        const int c = with[j / (CH / (8 * NT))], i = c * CH + (j % (CH / (8 * NT)) * NT + tid) * 8;
+      for (int j = wave; j < n; j += NW) {
         float v[8];
-        load_tokens<T, 8>(x, i, min(A.V, (c + 1) * CH), vec, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = next[e];
+        fetch(j + NW, next);
+        const int i = with[j] * SUB + lane * 8;
         uint32_t hit = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int b = bin_of(v[e], weigh.s, top);
+          const int b = G.bin(v[e]);
           if (b >= b0 && b <= b1 && key_of(v[e]) != 0) hit |= 1u << e;
         }
-        while (hit) {
-          const int e = __builtin_ctz(hit);
-          hit &= hit - 1;
-          const float q = to_f(x[i + e]);
-          const uint32_t at = atomicAdd(&ln, 1u);
-          if (at < CAP) list[at] = Token{place(key_of(q), i + e), fixed(weigh(q))};
-        }
+        if (__ballot(hit != 0) == 0) continue;
+        // the wave's tokens one behind the other
+        const uint32_t n_ = __popc(hit), upto = wave_scan(n_), all = lane_value(upto, 63);
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&ln, all);
+        at = lane_value(at, 0) + upto - n_;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (hit >> e & 1) {
+            if (at < CAP) list[at].place = place(key_of(v[e]), i + e);
+            ++at;
+          }
       }
       __syncthreads();
     }
+    uint32_t hi = 0, lo = 0xffffffffu;
+    for (uint32_t i = tid; i < ln; i += NT) {
+      const uint32_t k = (uint32_t)(list[i].place >> 32);
+      list[i].w = fixed(G.weight(value_of(k)));
+      hi = max(hi, k);
+      lo = min(lo, k);
+    }
+    hi = wave_max_u(hi);
+    lo = ~wave_max_u(~lo);
+    if (lane == 0 && hi) {
+      atomicMax(&kmax, hi);
+      atomicMin(&kmin, lo);
+    }
+    __syncthreads();
     return true;
   };
   // Of the listed tokens that are kept, in the order of falling places (or rising indexes, BY_INDEX): by count, the one
   // with `last` before it; by mass, the last one before which less than `room` lies.  `at`: its place; `mass`: up to and
   // with it.  The range of the order that holds it is cut into 256 parts until few tokens are left to be ranked.
-  constexpr int PER = CAP / NT;
   auto select = [&](bool by_index, bool by_mass, uint32_t last, unsigned long long room, unsigned long long& at,
                     unsigned long long& mass) {
     const uint32_t n = ln;
-    Token t[PER];
-    unsigned long long o[PER], hi = 0, lo = ~0ull;  // 0: none
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const uint32_t i = tid + e * NT;
-      t[e] = i < n ? list[i] : Token{0, 0};
-      o[e] = i < n && t[e].w ? (by_index ? t[e].place & 0xffffffffull : t[e].place) : 0;
-      if (o[e]) {
-        hi = max(hi, o[e]);
-        lo = min(lo, o[e]);
-      }
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      hi = max(hi, __shfl_xor(hi, d, 64));
-      lo = min(lo, __shfl_xor(lo, d, 64));
-    }
-    __syncthreads();  // what was before has been read
-    if (lane == 0) {
-      wmax[wave] = hi;
-      wmin[wave] = lo;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      hi = max(hi, wmax[w]);
-      lo = min(lo, wmin[w]);
-    }
     uint32_t n0 = 0, in = n;      // tokens and mass before the window, tokens in it
-    unsigned long long w0 = 0, width = hi - lo;
-    while (in > 32 && width > 0) {
+    unsigned long long w0 = 0;
+    // the window of the order: o in [hi - width, hi]
+    unsigned long long hi = by_index ? 0xffffffffull : (unsigned long long)kmax << 32 | 0xffffffffull;
+    unsigned long long width = by_index ? (unsigned long long)A.V - 1 : hi - ((unsigned long long)kmin << 32);
+    auto order = [&](const Token& t) { return by_index ? t.place & 0xffffffffull : t.place; };
+    auto inside = [&](const Token& t) { return t.w != 0 && order(t) <= hi && hi - order(t) <= width; };
+    __syncthreads();
+    while (in > 64 && width > 0) {
       const int sh = max(0, 64 - __builtin_clzll(width) - 8);
       if (tid < 256) {
         pcount[tid] = 0;
         pmass[tid] = 0;
       }
       __syncthreads();
-#pragma unroll
-      for (int e = 0; e < PER; ++e)
-        if (o[e] && o[e] <= hi && hi - o[e] <= width) {
-          const int q = (int)((hi - o[e]) >> sh);
+      for (uint32_t i = tid; i < n; i += NT)
+        if (inside(list[i])) {
+          const int q = (int)((hi - order(list[i])) >> sh);
           atomicAdd(&pcount[q], 1u);
-          atomicAdd(&pmass[q], t[e].w);
+          atomicAdd(&pmass[q], list[i].w);
         }
       __syncthreads();
       if (wave == 0) {
@@ -663,7 +747,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
           c[j] = cs += pcount[4 * lane + j];
           m[j] = ms += pmass[4 * lane + j];
         }
-        const uint32_t cb = wave_scan(cs) - cs, all = __shfl(cb + cs, 63, 64);
+        const uint32_t ce = wave_scan(cs), cb = ce - cs, all = lane_value(ce, 63);
         const unsigned long long mb = wave_scan(ms) - ms;
         int best = 255;
 #pragma unroll
@@ -674,8 +758,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
           pcount[4 * lane + j] = cb + c[j];
           pmass[4 * lane + j] = mb + m[j];
         }
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) best = min(best, __shfl_xor(best, d, 64));
+        best = 255 - (int)wave_max_u(255 - best);
         if (lane == 0) bsh = best;
       }
       __syncthreads();
@@ -688,53 +771,46 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
       width = min(width - ((unsigned long long)q << sh), (1ull << sh) - 1);
       __syncthreads();
     }
-    // the window's tokens, at most 32 of them (one, where its width is 0)
-    if (tid == 0) pcount[0] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < PER; ++e)
-      if (o[e] && o[e] <= hi && hi - o[e] <= width) {
-        const uint32_t i = atomicAdd(&pcount[0], 1u);
-        pmass[i] = o[e];
-        pmass[64 + i] = t[e].w;
-        pmass[128 + i] = t[e].place;
-      }
-    __syncthreads();
-    const uint32_t np = pcount[0];
-    unsigned long long best = 0, bp = 0, bm = 0;  // every thread looks them through: few, and one answer for all
+    // The window's tokens, at most 64 (places are all different), ranked by one wave: those within the cut are the
+    // first in the order, and the last of them has one less before it than they are.
+    if (n > 64) {
+      if (tid == 0) pcount[0] = 0;
+      __syncthreads();
+      for (uint32_t i = tid; i < n; i += NT)
+        if (inside(list[i])) {
+          const uint32_t j = atomicAdd(&pcount[0], 1u);
+          if (j < 64) {
+            pmass[j] = list[i].place;
+            pmass[64 + j] = list[i].w;
+          }
+        }
+      __syncthreads();
+    }
     if (wave == 0) {
-      const unsigned long long mine = lane < np ? pmass[lane] : 0, w = lane < np ? pmass[64 + lane] : 0;
-      uint32_t before = n0;
+      const uint32_t np = n > 64 ? min(pcount[0], 64u) : n;
+      Token t{0, 0};
+      if ((uint32_t)lane < np) t = n > 64 ? Token{pmass[lane], pmass[64 + lane]} : list[lane];
+      const bool have = t.w != 0;
+      const unsigned long long mine = order(t);
+      uint32_t rank = 0;
       unsigned long long m = w0;
-      for (uint32_t j = 0; j < np; ++j)
-        if (pmass[j] > mine) {
-          ++before;
-          m += pmass[64 + j];
-        }
-      const bool ok = lane < np && (by_mass ? m < room || before == 0 : before <= last);
-      best = ok ? ~mine : 0;  // the last of them: the smallest
-      bp = ok ? pmass[128 + lane] : 0;
-      bm = ok ? m + w : 0;
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1) {
-        const unsigned long long b2 = __shfl_xor(best, d, 64), p2 = __shfl_xor(bp, d, 64), m2 = __shfl_xor(bm, d, 64);
-        if (b2 > best) {
-          best = b2;
-          bp = p2;
-          bm = m2;
-        }
+      for (uint32_t j = 0; j < np; ++j) {
+        const unsigned long long w = lane_value(t.w, j);
+        const bool first = w != 0 && lane_value(mine, j) > mine;
+        rank += first;
+        m += first ? w : 0ull;
       }
-      if (lane == 0) {
-        wmax[0] = bp;
-        wmin[0] = bm;
+      const unsigned long long ok = __ballot(have && (by_mass ? m < room || n0 + rank == 0 : n0 + rank <= last));
+      if (have && rank + 1 == (uint32_t)__popcll(ok)) {
+        got[0] = t.place;
+        got[1] = m + t.w;
       }
     }
     __syncthreads();
-    at = wmax[0];
-    mass = wmin[0];
+    at = got[0];
+    mass = got[1];
   };
   auto whole = [](double w) -> unsigned long long { return w > 0.0 ? (unsigned long long)__builtin_ceil(w) : 0ull; };
-  const double ym = (double)value_of(mk) * weigh.s + log2(S.m);  // min-p's border
   // first bin whose tokens take the mass to the goal
   auto bin_at = [&](double goal) -> int {
     __syncthreads();
@@ -752,10 +828,10 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     bk = bsh;
   }
   if (S.m > 0.0) {
-    const double d = top - floor(ym * 8.0);
+    const double d = G.top - floor((double)value_of(mk) * G.s8 + 8.0 * log2(S.m));
     bm = d < (double)(NB - 1) ? max((int)d, 0) : (d != d ? 0 : NB - 1);
   }
-  auto weight_of = [&](const Token& t) { return weigh(value_of((uint32_t)(t.place >> 32))); };
+  const double least = S.m * wmax;  // by min-p
   // Drops what min-p or a place cuts off the list; returns the mass that is left
   auto keep = [&](unsigned long long tp) -> unsigned long long {
     __syncthreads();
@@ -763,7 +839,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     __syncthreads();
     unsigned long long w = 0;
     for (uint32_t i = tid; i < ln; i += NT) {
-      if (list[i].place < tp || !(weight_of(list[i]) >= S.m)) list[i].w = 0;
+      if (list[i].place < tp || !(G.weight(value_of((uint32_t)(list[i].place >> 32))) >= least)) list[i].w = 0;
       w += list[i].w;
     }
     w = wave_add(w);
@@ -775,8 +851,9 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   // Steps: the end of top-k's set, the end of top-p's, and with few candidates, all of them on the list, the draw;
   // else on one border's bin at a time.  (One loop: the selection's code is there once.)
   const bool nucleus = S.p < 1.0 && S.p > 0.0;
+  const double enough = S.p * (1.0 - 0x1p-40);  // masses are good to 2^-45 or so: one that meets p exactly has to reach it
   int bc = bk;  // candidates: up to this bin; top-k's border is in the list where top-p's goal needs its set's mass
-  if (!(topk && nucleus)) bc = min(min(bk, bm), S.p < 1.0 ? (nucleus ? bin_at(S.p * cmass[NB - 1]) : 0) : NB - 1);
+  if (!(topk && nucleus)) bc = min(min(bk, bm), S.p < 1.0 ? (nucleus ? bin_at(enough * cmass[NB - 1]) : 0) : NB - 1);
   const bool few = bc < NB - 1 && cum[bc] <= CAP;
   int bt = bk;                  // bin of the last token that top-k and top-p keep; NB - 1: none with mass is cut
   unsigned long long tp = 0;    // its place
@@ -794,7 +871,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     int b = bt;
     if (step == 1) {
       if (!nucleus) continue;
-      const double goal = S.p * set;
+      const double goal = enough * set;
       if (!few) {
         b = min(bin_at(goal), bt);
         if (b == NB - 1) continue;
@@ -818,7 +895,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     if (step == 2) {
       if (tid == 0) {
         A.ids[r] = (int64_t)(0xffffffffu - (uint32_t)q);
-        A.probs[r] = (float)(weigh(value_of((uint32_t)(q >> 32))) / ((double)sum * (1.0 / kFix)));
+        A.probs[r] = (float)(G.weight(value_of((uint32_t)(q >> 32))) / ((double)sum * (1.0 / kFix)));
       }
       return;
     }
@@ -833,15 +910,18 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     radix_row<T>(A, r, mk, valid, S);
     return;
   }
-  auto passes = [&](unsigned long long at, double w) { return at >= tp && w >= S.m; };
+  auto passes = [&](unsigned long long at, double w) { return at >= tp && w >= least; };
   const double part = partial ? (double)keep(tp) * (1.0 / kFix) : 0.0;
   const double total = (bf > 0 ? cmass[bf - 1] : 0.0) + part, goal = S.u * total;
 
   // the chunk in which the kept mass passes the goal: a wave sums a chunk's whole bins and its listed tokens
   double run = 0.0, start = 0.0, lastrun = 0.0;
   int at = -1, lastc = -1;
+  double scale[NB / 64];  // of this lane's bins of a chunk, before its shift
+#pragma unroll
+  for (int j = 0; j < NB / 64; ++j) scale[j] = exp2_64(-0.125 * (double)(lane + 64 * j + 1)) * (1.0 / kPart);
   for (int c0 = 0; c0 < nc && at < 0; c0 += NW) {
-    if (nc > MC && c0 % MC == 0) scales(c0);
+    if (nc > MC && c0 % MC == 0) shifts(c0);
     const int c = c0 + wave;
     double w = 0.0;
     if (c < nc) {
@@ -849,9 +929,9 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
 #pragma unroll
       for (int j = 0; j < NB / 64; ++j) {
         const int b = lane + 64 * j;
-        w += b < hi ? (double)C[c].mass[b] : 0.0;
+        w += b < hi ? (double)C[c].mass[b] * scale[j] : 0.0;
       }
-      w *= scale[c % MC];
+      w *= exp2_64(-0.125 * (double)shift[c % MC]);
       if (partial) {
         unsigned long long f = 0;
         for (uint32_t j = lane; j < ln; j += 64)
@@ -883,17 +963,23 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   }
   // Scan of that chunk: the waves' parts, then the part in which the goal is passed, 64 tokens at a time
   const int i0 = at * CH + wave * (CH / NW), i1 = min(A.V, i0 + CH / NW);
-  auto mass_of = [&](int i) -> double {
-    const float q = i < i1 ? to_f(x[i]) : -INFINITY;
+  auto mass_of = [&](int i, float q) -> double {
     const uint32_t k = key_of(q);
-    const int b = k != 0 ? bin_of(q, weigh.s, top) : NB;
+    const int b = k != 0 ? G.bin(q) : NB;
     if (!(b < bf || (partial && b == bf))) return 0.0;
-    const double w = weigh(q);
+    const double w = G.weight(q);
     return b < bf || passes(place(k, i), w) ? w : 0.0;
   };
+  auto token = [&](int i) { return i < i1 ? to_f(x[i]) : -INFINITY; };
   double sum = 0.0;
 #pragma unroll 1
-  for (int i = i0 + lane; i < i1; i += 64) sum += mass_of(i);
+  for (int i = i0 + lane; i - lane < i1; i += 256) {
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = token(i + 64 * j);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum += mass_of(i + 64 * j, q[j]);
+  }
   sum = wave_add(sum);
   __syncthreads();
   if (lane == 0) red[wave] = sum;
@@ -912,17 +998,20 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   if (wave != mine) return;
   int found = i0;
   double share = 0.0;
+  float next = token(i0 + lane);
 #pragma unroll 1
   for (int i = i0; i < i1; i += 64) {
-    const double w = mass_of(i + lane), c = wave_scan(w);
+    const float q = next;
+    next = token(i + 64 + lane);
+    const double w = mass_of(i + lane, q), c = wave_scan(w);
     const unsigned long long any = __ballot(w > 0.0), hit = __ballot(w > 0.0 && from + c > goal);
     if (any) {
       const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);  // (rounding: the last with mass)
       found = i + l;
-      share = __shfl(w, l, 64);
+      share = lane_value(w, l);
       if (hit) break;
     }
-    from += __shfl(c, 63, 64);
+    from += lane_value(c, 63);
   }
   if (lane == 0) {
     A.ids[r] = found;
@@ -945,7 +1034,9 @@ PA_API int pa_sample(const void* x, long long row, int rows, int V, const void* 
                      int64_t* ids, float* probs, void* ws, int dt, hipStream_t st) {
   if (rows == 0) return 0;
   if (rows < 0 || V <= 0 || V > (1 << 30) || !u || !ids || !probs || !ws) return (int)hipErrorInvalidValue;
-  pa::smp::Args A{x, row, V, u, u64, t, k, p, m, t0, p0, m0, k0, ids, probs};
+  const float* const none = (const float*)ws;  // at least a number for every row
+  pa::smp::Args A{x, row, V, u, u64, t ? t : none, k ? k : (const int*)none, p ? p : none, m ? m : none, t0, p0, m0, k0,
+                  (t ? 1 : 0) | (k ? 2 : 0) | (p ? 4 : 0) | (m ? 8 : 0), ids, probs};
   const int nc = (V + pa::smp::CH - 1) / pa::smp::CH;
   if (rows * (long long)nc > 0x7fffffff) return (int)hipErrorInvalidValue;
   pa::smp::Chunk* C = (pa::smp::Chunk*)ws;
