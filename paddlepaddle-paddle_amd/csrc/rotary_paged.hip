@@ -8,10 +8,12 @@
 // turn in 64 bits (at position 10^6 a 32-bit angle is off by 0.03 radian), its sine and cosine and the
 // rotation are 32-bit, and each output is rounded once.
 //
-// What bounds it: memory traffic (every value read and written once).  So: 16-byte accesses; one launch
-// for queries and keys (and values, where they go to the pages); a block takes 1 or 4 tokens, forms
-// their R/2 angles once in LDS and uses them for every head, so the 64-bit arithmetic is paid per token
-// and pair and not per head.
+// What bounds it: memory traffic (every value read and written once).  So: 16-byte accesses; one launch for queries
+// and keys (and values, where they go to the pages); a block for a token, which forms its R/2 angles once in LDS and
+// uses them for every head, so the 64-bit arithmetic is paid per token and pair and not per head.  The first loads are
+// on their way before the angles (and the token's place in the pages: three dependent loads) are known; with that,
+// blocks of 2 to 4 tokens are slower (0.61 GB of queries and keys in bf16: 67 us with one token a block, 69 with 2 or 4;
+// 8340 tokens to pages of 16: 31, 35, 39 us).
 #include "common.h"
 
 namespace pa {
@@ -19,41 +21,50 @@ namespace rot {
 
 constexpr int kMaxPairs = 256;  // R / 2 of one token
 
-// cos/sin of a position's pairs: from frequencies, or from tables[(b, p, i)] of the given length
-struct Angles {
-  const double* inv_freq;
-  const float* cos_t;
-  const float* sin_t;
-  long long tab_b;  // table stride of a sequence
-  int tab_len;      // positions per table
-  float scale;
-};
-
-__device__ __forceinline__ float2 angle(const Angles& a, int b, long long p, int i, int pairs, float sign) {
+__device__ __forceinline__ float2 angle(const double* inv_freq, float scale, long long p, int i, float sign) {
   float c, s;
-  if (a.cos_t != nullptr) {
-    if (p < 0 || p >= a.tab_len) return make_float2(NAN, NAN);  // no such row: loud, and never read
-    const long long o = (long long)b * a.tab_b + p * pairs + i;
-    c = a.cos_t[o];
-    s = a.sin_t[o];
-  } else {
-    const double turns = (double)p * a.inv_freq[i] * 0.15915494309189533577;  // / 2 pi
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    c *= a.scale;
-    s *= a.scale;
-  }
-  return make_float2(c, sign * s);
+  const double turns = (double)p * inv_freq[i] * 0.15915494309189533577;  // / 2 pi
+  sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+  return make_float2(c * scale, sign * s * scale);
 }
 
-// One vector unit of a head: V values (interleaved pairs, or values that are copied), or the V values at
-// x and their V partners at x + half.  No contraction: a product is rounded before it is added, as in
-// the composite of elementary operations.
+// Units of a head: `nr` that turn (V values and their V partners at + pairs in the half layout, V values of
+// interleaved pairs), then the copied ones of V values.  A thread's units of the block's token, in order:
+struct Walk {
+  int units, nr, heads, Ht;  // heads: taken at once
+  int u, hh, hl;             // the next unit, its head
+  bool more;
+  __device__ __forceinline__ Walk(int V, bool inter, int D, int pairs, int Ht_) {
+    nr = (inter ? 2 * pairs : pairs) / V;
+    units = nr + (D - 2 * pairs) / V;
+    heads = units < 256 ? 256 / units : 1;
+    Ht = Ht_;
+    hl = threadIdx.x / units;
+    u = threadIdx.x % units;
+    hh = hl;
+    more = hl < heads && hl < Ht;
+  }
+  __device__ __forceinline__ void next() {
+    hh += heads;
+    if (hh < Ht) return;
+    hh = hl;
+    u += 256;  // only where a head has over 256 units
+    more = u < units;
+  }
+  template <int V, bool INTER>
+  __device__ __forceinline__ int off(int pairs) const {
+    return INTER || u < nr ? u * V : 2 * pairs + (u - nr) * V;
+  }
+};
+
+// One unit turned (or copied), with the bias on it.
 template <typename T, int V, bool INTER>
-__device__ __forceinline__ void turn_unit(const T* __restrict__ x, T* __restrict__ y, const T* __restrict__ bias,
-                                          const float2* __restrict__ cs, int half, bool turn, bool two) {
-#pragma clang fp contract(off)
+__device__ __forceinline__ void turn_unit(const Pack<T, V>& x, const Pack<T, V>& x2, T* __restrict__ y,
+                                          const T* __restrict__ bias, const float2* __restrict__ cs, int half, bool turn,
+                                          bool two) {
   float a[V], b[V];
-  load_f<T, V>(x, a);
+#pragma unroll
+  for (int e = 0; e < V; ++e) a[e] = to_f(x.v[e]);
   if (bias) {
     float t[V];
     load_f<T, V>(bias, t);
@@ -73,7 +84,8 @@ __device__ __forceinline__ void turn_unit(const T* __restrict__ x, T* __restrict
     store_f<T, V>(y, a);
   } else {
     if (two) {
-      load_f<T, V>(x + half, b);
+#pragma unroll
+      for (int e = 0; e < V; ++e) b[e] = to_f(x2.v[e]);
       if (bias) {
         float t[V];
         load_f<T, V>(bias + half, t);
@@ -95,11 +107,32 @@ __device__ __forceinline__ void turn_unit(const T* __restrict__ x, T* __restrict
   }
 }
 
-// Units of a head: `nr` that turn (each V values and their partners in the half layout, V values
-// interleaved), then the copied ones.  Offset of unit u within the head:
-template <int V, bool INTER>
-__device__ __forceinline__ int unit_off(int u, int nr, int pairs) {
-  return INTER ? u * V : (u < nr ? u * V : 2 * pairs + (u - nr) * V);
+// A block's units, G loads of a thread in flight; the first ones are on their way while `before` forms the angles.
+template <typename T, int V, bool INTER, int G, typename Src, typename Before, typename Put>
+__device__ __forceinline__ void stream(Walk w, int pairs, Src src, Before before, Put put) {
+  Pack<T, V> a[G], b[G];
+  Walk ahead = w;
+  auto load = [&]() {
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+      if (ahead.more) {
+        const T* x = src(ahead.hh) + ahead.template off<V, INTER>(pairs);
+        a[j] = *reinterpret_cast<const Pack<T, V>*>(x);
+        if (!INTER && ahead.u < w.nr) b[j] = *reinterpret_cast<const Pack<T, V>*>(x + pairs);
+        ahead.next();
+      }
+  };
+  load();
+  before();
+  while (w.more) {
+#pragma unroll
+    for (int j = 0; j < G; ++j)
+      if (w.more) {
+        put(w.hh, w.template off<V, INTER>(pairs), w.u < w.nr, a[j], b[j]);
+        w.next();
+      }
+    load();
+  }
 }
 
 struct RopeArgs {
@@ -112,44 +145,34 @@ struct RopeArgs {
   int pos64;
   int S, D, pairs;
   long long tokens;
-  float sign;
-  Angles ang;
+  float sign, scale;
+  const double* inv_freq;
 };
 
 template <typename T, int V, bool INTER>
-__global__ __launch_bounds__(256) void rope_kernel(RopeArgs A, int per_block) {
-  __shared__ float2 cs[4][kMaxPairs];
-  const long long t0 = (long long)blockIdx.x * per_block;
-  const int nt = (int)min((long long)per_block, A.tokens - t0);
-  for (int i = threadIdx.x; i < nt * A.pairs; i += 256) {
-    const int t = i / A.pairs, j = i - t * A.pairs;
-    const long long tok = t0 + t, b = tok / A.S, s = tok - b * A.S;
-    long long p = s;
-    if (A.pos)
-      p = A.pos64 ? reinterpret_cast<const int64_t*>(A.pos)[b * A.ps[0] + s * A.ps[1]]
-                  : (long long)reinterpret_cast<const int32_t*>(A.pos)[b * A.ps[0] + s * A.ps[1]];
-    cs[t][j] = angle(A.ang, 0, p, j, A.pairs, A.sign);
-  }
-  __syncthreads();
-  const int nr = INTER ? 2 * A.pairs / V : A.pairs / V;
-  const int units = nr + (A.D - 2 * A.pairs) / V;
-  const int Ht = A.H[0] + A.H[1];
-  const int heads = 256 / units > 0 ? 256 / units : 1;  // heads that the block takes at once
-  const int hl = threadIdx.x / units;
-  for (int u = threadIdx.x % units; u < units; u += 256) {  // more than once only where a head has over 256 units
-    const int off = unit_off<V, INTER>(u, nr, A.pairs);
-    if (hl >= heads) break;
-    for (int t = 0; t < nt; ++t) {
-      const long long tok = t0 + t, b = tok / A.S, s = tok - b * A.S;
-      for (int hh = hl; hh < Ht; hh += heads) {
-        const int w = hh < A.H[0] ? 0 : 1, h = w ? hh - A.H[0] : hh;
-        const T* x = reinterpret_cast<const T*>(w ? A.x[1] : A.x[0]) + b * (w ? A.xs[1][0] : A.xs[0][0]) +
-                     s * (w ? A.xs[1][1] : A.xs[0][1]) + h * (w ? A.xs[1][2] : A.xs[0][2]) + off;
-        T* y = reinterpret_cast<T*>(w ? A.y[1] : A.y[0]) + (tok * (w ? A.H[1] : A.H[0]) + h) * (long long)A.D + off;
-        turn_unit<T, V, INTER>(x, y, (const T*)nullptr, &cs[t][INTER ? off / 2 : off], A.pairs, u < nr, u < nr);
-      }
-    }
-  }
+__global__ __launch_bounds__(256) void rope_kernel(RopeArgs A) {
+  __shared__ float2 cs[kMaxPairs];
+  const long long tok = blockIdx.x;
+  const int b = blockIdx.x / A.S, s = blockIdx.x - b * A.S;
+  const T* const x0 = reinterpret_cast<const T*>(A.x[0]) + b * A.xs[0][0] + s * A.xs[0][1];
+  const T* const x1 = reinterpret_cast<const T*>(A.x[1]) + b * A.xs[1][0] + s * A.xs[1][1];
+  T* const y0 = reinterpret_cast<T*>(A.y[0]) + tok * A.H[0] * A.D;
+  T* const y1 = reinterpret_cast<T*>(A.y[1]) + tok * A.H[1] * A.D;
+  stream<T, V, INTER, 4>(
+      Walk(V, INTER, A.D, A.pairs, A.H[0] + A.H[1]), A.pairs,
+      [&](int hh) { return hh < A.H[0] ? x0 + hh * A.xs[0][2] : x1 + (hh - A.H[0]) * A.xs[1][2]; },
+      [&]() {
+        long long p = s;
+        if (A.pos)
+          p = A.pos64 ? reinterpret_cast<const int64_t*>(A.pos)[b * A.ps[0] + s * A.ps[1]]
+                      : (long long)reinterpret_cast<const int32_t*>(A.pos)[b * A.ps[0] + s * A.ps[1]];
+        for (int i = threadIdx.x; i < A.pairs; i += 256) cs[i] = angle(A.inv_freq, A.scale, p, i, A.sign);
+        __syncthreads();
+      },
+      [&](int hh, int off, bool turn, const Pack<T, V>& a, const Pack<T, V>& b) {
+        T* y = (hh < A.H[0] ? y0 + (long long)hh * A.D : y1 + (long long)(hh - A.H[0]) * A.D) + off;
+        turn_unit<T, V, INTER>(a, b, y, (const T*)nullptr, &cs[INTER ? off / 2 : off], A.pairs, turn, turn);
+      });
 }
 
 struct AppendArgs {
@@ -168,88 +191,69 @@ struct AppendArgs {
   const int* off_dev;
   long long off;  // position = off + place in the cache
   int T, B, Hq, Hkv, D, pairs;
-  Angles ang;
+  float scale;
+  const double* inv_freq;
 };
 
-// largest b with cu[b] <= t, or B where t lies behind the last sequence (-1 before the first)
+// Largest b with cu[b] <= t: B behind the last sequence, -1 before the first.  By a whole wave, 64 borders a step.
 __device__ __forceinline__ int seq_of_token(const int* cu, int B, int t) {
-  if (t >= cu[B]) return B;
-  int lo = -1, hi = B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
+  int lo = 0, n = B + 1;  // cu[0 .. lo) are <= t, cu[lo + n ..) are not
+  while (n > 0) {
+    const int step = (n + 63) / 64, i = (int)(threadIdx.x & 63) * step + step - 1;  // (a step's last border)
+    const int full = __popcll(__ballot(i < n && cu[lo + i] <= t));
+    lo += full * step;
+    n = step > 1 ? min(step - 1, n - full * step) : 0;
   }
-  return lo;
+  return lo - 1;
 }
 
 template <typename T, int V, bool INTER>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs A, int per_block) {
-  __shared__ float2 cs[4][kMaxPairs];
-  __shared__ long long dst[4];  // where the token's keys go (element offset of head 0), -1: nowhere
-  __shared__ long long where[4];
-  __shared__ int seq[4];
-  const int t0 = blockIdx.x * per_block, nt = min(per_block, A.T - t0);
-  if (threadIdx.x < nt) {
-    const int t = t0 + threadIdx.x;
-    const int b = A.cu ? seq_of_token(A.cu, A.B, t) : (t < A.B ? t : A.B);
-    long long d = -1, p = 0;
-    int s = -1;
-    if (b >= 0 && b < A.B) {
-      s = b;
-      p = (long long)A.lens[b] + (A.cu ? t - A.cu[b] : 0);
-      const long long pg = p / A.page;
-      if (p >= 0 && pg < A.max_blocks) {
-        const int blk = A.tables[(long long)b * A.tstride + pg];
-        if (blk >= 0 && blk < A.num_blocks) d = blk * A.cs[0] + (p - pg * A.page) * A.cs[2];
-      }
-      p += A.off_dev ? (long long)*A.off_dev : A.off;
-    }
-    dst[threadIdx.x] = d;
-    where[threadIdx.x] = p;
-    seq[threadIdx.x] = s;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < nt * A.pairs; i += 256) {
-    const int t = i / A.pairs, j = i - t * A.pairs;
-    if (seq[t] >= 0) cs[t][j] = angle(A.ang, seq[t], where[t], j, A.pairs, 1.f);
-  }
-  __syncthreads();
-  const int nr = INTER ? 2 * A.pairs / V : A.pairs / V;
-  const int units = nr + (A.D - 2 * A.pairs) / V;
-  const int Ht = A.Hq + 2 * A.Hkv;
-  const int heads = 256 / units > 0 ? 256 / units : 1;
-  const int hl = threadIdx.x / units;
-  for (int u = threadIdx.x % units; u < units; u += 256) {
-    const int off = unit_off<V, INTER>(u, nr, A.pairs);
-    if (hl >= heads) break;
-    for (int t = 0; t < nt; ++t) {
-      const long long tok = t0 + t;
-      for (int hh = hl; hh < Ht; hh += heads) {
-        const long long o = (long long)hh * A.D + off;
-        const T* x = reinterpret_cast<const T*>(A.qkv) + tok * A.row + o;
-        const T* bias = A.bias ? reinterpret_cast<const T*>(A.bias) + o : nullptr;
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs A) {
+  __shared__ float2 cs[kMaxPairs];
+  const int t = blockIdx.x;
+  const T* const x = reinterpret_cast<const T*>(A.qkv) + (long long)t * A.row;
+  T* const q = reinterpret_cast<T*>(A.q) + (long long)t * A.Hq * A.D;
+  bool in = false;     // the token belongs to a sequence
+  long long dst = -1;  // where its keys go (element offset of head 0), -1: nowhere
+  stream<T, V, INTER, 4>(
+      Walk(V, INTER, A.D, A.pairs, A.Hq + 2 * A.Hkv), A.pairs, [&](int hh) { return x + (long long)hh * A.D; },
+      [&]() {
+        // (each wave for itself: no barrier before the angles)
+        const int b = A.cu ? __builtin_amdgcn_readfirstlane(seq_of_token(A.cu, A.B, t)) : (t < A.B ? t : A.B);
+        in = b >= 0 && b < A.B;
+        if (in) {
+          long long p = (long long)A.lens[b] + (A.cu ? t - A.cu[b] : 0);
+          const long long pg = p / A.page;
+          if (p >= 0 && pg < A.max_blocks) {
+            const int blk = A.tables[(long long)b * A.tstride + pg];
+            if (blk >= 0 && blk < A.num_blocks) dst = blk * A.cs[0] + (p - pg * A.page) * A.cs[2];
+          }
+          p += A.off_dev ? (long long)*A.off_dev : A.off;
+          for (int i = threadIdx.x; i < A.pairs; i += 256) cs[i] = angle(A.inv_freq, A.scale, p, i, 1.f);
+        }
+        __syncthreads();
+      },
+      [&](int hh, int off, bool turn, const Pack<T, V>& a, const Pack<T, V>& b) {
         T* y;
         if (hh < A.Hq) {
-          y = reinterpret_cast<T*>(A.q) + (tok * A.Hq + hh) * (long long)A.D + off;
-          if (seq[t] < 0) {  // behind the last sequence
+          y = q + (long long)hh * A.D + off;
+          if (!in) {  // behind the last sequence
             float z[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) z[e] = 0.f;
             store_f<T, V>(y, z);
-            if (!INTER && u < nr) store_f<T, V>(y + A.pairs, z);
-            continue;
+            if (!INTER && turn) store_f<T, V>(y + A.pairs, z);
+            return;
           }
         } else {
-          if (dst[t] < 0) continue;
+          if (dst < 0) return;
           const bool isv = hh >= A.Hq + A.Hkv;
           const int h = hh - A.Hq - (isv ? A.Hkv : 0);
-          y = reinterpret_cast<T*>(isv ? A.vc : A.kc) + dst[t] + h * A.cs[1] + off;
+          y = reinterpret_cast<T*>(isv ? A.vc : A.kc) + dst + h * A.cs[1] + off;
         }
-        turn_unit<T, V, INTER>(x, y, bias, &cs[t][INTER ? off / 2 : off], A.pairs, u < nr && hh < A.Hq + A.Hkv, u < nr);
-      }
-    }
-  }
+        const T* bias = A.bias ? reinterpret_cast<const T*>(A.bias) + (long long)hh * A.D + off : nullptr;
+        turn_unit<T, V, INTER>(a, b, y, bias, &cs[INTER ? off / 2 : off], A.pairs, turn && hh < A.Hq + A.Hkv, turn);
+      });
 }
 
 // Vector width: the widest of 16, 8, 4 ... bytes that divides the pairs, the copied part and, by the
@@ -277,10 +281,6 @@ using namespace pa::rot;
     else KERNEL<T, 1, false> __VA_ARGS__;                                                        \
   }
 
-// Tokens per block: 4 once that still gives every CU two blocks (the angles of 4 tokens fill the
-// block's 256 threads at R = 128), else 1, which spreads a decode step over the chip.
-static int rot_tokens_per_block(long long tokens) { return tokens >= 2048 ? 4 : 1; }
-
 // q / k: [B, S, H, D] views with unit inner stride and the given (batch, token, head) strides; yq / yk
 // contiguous.  `align`: elements that divide every stride and address.  sign -1: the backward pass.
 PA_API int pa_rope_freq(const void* q, const void* k, void* yq, void* yk, const long long* qs, const long long* ks,
@@ -295,27 +295,24 @@ PA_API int pa_rope_freq(const void* q, const void* k, void* yq, void* yk, const 
   A.H[0] = Hq; A.H[1] = k ? Hk : 0;
   A.pos = pos; A.ps[0] = pos_b; A.ps[1] = pos_s; A.pos64 = pos64;
   A.S = S; A.D = D; A.pairs = pairs; A.tokens = (long long)B * S; A.sign = sign;
-  A.ang = Angles{inv_freq, nullptr, nullptr, 0, 0, scale};
+  A.inv_freq = inv_freq; A.scale = scale;
   if (A.tokens == 0 || A.H[0] + A.H[1] == 0) return 0;
   const int v = width(dt == 0 ? 4 : 2, D, pairs, inter != 0, align);
   if (inter && (D % v || align % v)) return (int)hipErrorInvalidValue;  // pairs are loaded together
-  const int pb = rot_tokens_per_block(A.tokens);
-  const long long grid = (A.tokens + pb - 1) / pb;
-  if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
-  PA_DISPATCH_DTYPE(dt, T, PA_ROT_LAUNCH(T, rope_kernel, <<<(int)grid, 256, 0, st>>>(A, pb)))
+  if (A.tokens > 0x7fffffff) return (int)hipErrorInvalidValue;
+  PA_DISPATCH_DTYPE(dt, T, PA_ROT_LAUNCH(T, rope_kernel, <<<(int)A.tokens, 256, 0, st>>>(A)))
   return (int)hipGetLastError();
 }
 
 // qkv rows [T, (Hq + 2 Hkv) D] (+ bias) -> q [T, Hq, D] turned, keys (turned) and values into the pages.
-// Angles from inv_freq (position = off or *off_dev + place), or from cos / sin tables [B, tab_len, pairs].
+// The angle's position: off or *off_dev, + place.
 PA_API int pa_paged_append(const void* qkv, long long row, const void* bias, void* q, void* kc, void* vc,
                            const long long* cstr, const int* tables, long long tstride, int max_blocks, int num_blocks,
                            int page, const int* lens, const int* cu, const int* off_dev, long long off, int T, int B,
                            int Hq, int Hkv, int D, int pairs, int inter, const double* inv_freq, float scale,
-                           const float* cos_t, const float* sin_t, long long tab_b, int tab_len, int align, int dt,
-                           hipStream_t st) {
+                           int align, int dt, hipStream_t st) {
   if (T < 0 || B < 0 || Hq < 0 || Hkv <= 0 || D <= 0 || pairs < 0 || 2 * pairs > D || pairs > kMaxPairs || page <= 0 ||
-      align < 1 || (pairs > 0 && !inv_freq && !(cos_t && sin_t)))
+      align < 1 || (pairs > 0 && !inv_freq))
     return (int)hipErrorInvalidValue;
   if (T == 0) return 0;
   AppendArgs A;
@@ -324,10 +321,9 @@ PA_API int pa_paged_append(const void* qkv, long long row, const void* bias, voi
   A.tables = tables; A.tstride = tstride; A.max_blocks = max_blocks; A.num_blocks = num_blocks; A.page = page;
   A.lens = lens; A.cu = cu; A.off_dev = off_dev; A.off = off;
   A.T = T; A.B = B; A.Hq = Hq; A.Hkv = Hkv; A.D = D; A.pairs = pairs;
-  A.ang = Angles{inv_freq, cos_t, sin_t, tab_b, tab_len, scale};
+  A.inv_freq = inv_freq; A.scale = scale;
   const int v = width(dt == 0 ? 4 : 2, D, pairs, inter != 0, align);
   if (inter && (D % v || align % v)) return (int)hipErrorInvalidValue;
-  const int pb = rot_tokens_per_block(T);
-  PA_DISPATCH_DTYPE(dt, T_, PA_ROT_LAUNCH(T_, append_kernel, <<<(T + pb - 1) / pb, 256, 0, st>>>(A, pb)))
+  PA_DISPATCH_DTYPE(dt, T_, PA_ROT_LAUNCH(T_, append_kernel, <<<T, 256, 0, st>>>(A)))
   return (int)hipGetLastError();
 }

@@ -928,7 +928,7 @@ def blha_get_max_len(seq_lens_encoder, seq_lens_decoder, batch_size):
 # ------------------------------------------------------- a serving step over a paged KV cache
 def _check(ok, name, what):
     if not ok:
-        raise ValueError(f"{name}: {what}")
+        raise ValueError(f"{name}: {what() if callable(what) else what}")
 
 
 def _same_device(name, first, **others):
@@ -939,10 +939,10 @@ def _same_device(name, first, **others):
 
 def _int32(name, what, t, shape):
     t = _u(t)
-    _check(isinstance(t, torch.Tensor) and t.dtype in (torch.int32, torch.int64), name, f"{what} must be an integer tensor")
+    _check(isinstance(t, torch.Tensor) and t.dtype in (torch.int32, torch.int64), name, lambda: f"{what} must be an integer tensor")
     _check(t.dim() == len(shape) and all(n is None or n == m for n, m in zip(shape, t.shape)), name,
-           f"{what} must have shape {list(shape)}, got {list(t.shape)}")
-    return t.to(torch.int32).contiguous()
+           lambda: f"{what} must have shape {list(shape)}, got {list(t.shape)}")
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def _frequencies(name, inv_freq, D, interleaved):
@@ -950,9 +950,9 @@ def _frequencies(name, inv_freq, D, interleaved):
     _check(isinstance(f, torch.Tensor) and f.dim() == 1 and f.dtype in (torch.float32, torch.float64), name,
            "inv_freq must be a one-dimensional float32 or float64 tensor")
     _check(2 * f.numel() <= D and f.numel() <= ops.rotary_paged.MAX_PAIRS, name,
-           f"{f.numel()} frequencies turn {2 * f.numel()} values of a head: it has {D}, and at most "
+           lambda: f"{f.numel()} frequencies turn {2 * f.numel()} values of a head: it has {D}, and at most "
            f"{2 * ops.rotary_paged.MAX_PAIRS} can be turned")
-    _check(not interleaved or D % 2 == 0, name, f"interleaved pairs need an even head dim, got {D}")
+    _check(not interleaved or D % 2 == 0, name, lambda: f"interleaved pairs need an even head dim, got {D}")
     return f
 
 
@@ -970,20 +970,20 @@ def rotary_inv_freq(rotary_dim, base=10000.0, scaling=None):
     overrides it)."""
     name = 'rotary_inv_freq'
     R = int(rotary_dim)
-    _check(R > 0 and R % 2 == 0, name, f"rotary_dim must be even and positive, got {rotary_dim}")
-    _check(base > 0, name, f"base must be positive, got {base}")
+    _check(R > 0 and R % 2 == 0, name, lambda: f"rotary_dim must be even and positive, got {rotary_dim}")
+    _check(base > 0, name, lambda: f"base must be positive, got {base}")
     i = torch.arange(0, R, 2, dtype=torch.float64) / R
     f, out_scale = float(base) ** -i, 1.0
     if scaling is not None:
         kind, factor = scaling.get('type'), float(scaling.get('factor', 1.0))
-        _check(factor > 0, name, f"factor must be positive, got {factor}")
+        _check(factor > 0, name, lambda: f"factor must be positive, got {factor}")
         if kind == 'linear':
             f = f / factor
         elif kind == 'ntk':
             _check(R > 2, name, "ntk scaling needs rotary_dim > 2")
             f = (float(base) * factor ** (R / (R - 2))) ** -i
         elif kind in ('wavelength', 'yarn'):
-            _check(scaling.get('original_max_position', 0) > 0, name, f"{kind} scaling needs original_max_position")
+            _check(scaling.get('original_max_position', 0) > 0, name, lambda: f"{kind} scaling needs original_max_position")
             span = float(scaling['original_max_position'])
             if kind == 'wavelength':
                 lo, hi = float(scaling.get('low_freq_factor', 1.0)), float(scaling.get('high_freq_factor', 4.0))
@@ -1016,14 +1016,14 @@ def fused_partial_rotary_embedding(q, k=None, inv_freq=None, position_ids=None, 
     (k None if not given)."""
     name = 'fused_partial_rotary_embedding'
     a, b = _u(q), _u(k) if k is not None else None
-    _check(a.dim() in (3, 4), name, f"q must be [B, S, H, D] or [T, H, D], got {list(a.shape)}")
-    _check(a.dtype in ops.rotary_paged.FLOATS, name, f"unsupported type {a.dtype}")
+    _check(a.dim() in (3, 4), name, lambda: f"q must be [B, S, H, D] or [T, H, D], got {list(a.shape)}")
+    _check(a.dtype in ops.rotary_paged.FLOATS, name, lambda: f"unsupported type {a.dtype}")
     f = _frequencies(name, inv_freq, a.shape[-1], interleaved)
     _same_device(name, a, k=b, inv_freq=f, position_ids=_u(position_ids))
     if b is not None:
-        _check(b.dtype == a.dtype, name, f"q is {a.dtype}, k {b.dtype}")
+        _check(b.dtype == a.dtype, name, lambda: f"q is {a.dtype}, k {b.dtype}")
         _check(b.dim() == a.dim() and b.shape[:-2] == a.shape[:-2] and b.shape[-1] == a.shape[-1], name,
-               f"k must be like q but for its heads, got {list(b.shape)} beside {list(a.shape)}")
+               lambda: f"k must be like q but for its heads, got {list(b.shape)} beside {list(a.shape)}")
     packed = a.dim() == 3
     if packed:
         a, b = a[None], None if b is None else b[None]
@@ -1034,7 +1034,7 @@ def fused_partial_rotary_embedding(q, k=None, inv_freq=None, position_ids=None, 
         _check(pos.dtype in (torch.int32, torch.int64), name, "position_ids must be integers")
         pos = pos[None] if pos.dim() == 1 else pos
         _check(pos.dim() == 2 and pos.shape[0] in (1, B) and pos.shape[1] == S, name,
-               f"position_ids must be [{B}, {S}], [1, {S}] or [{S}], got {list(_u(position_ids).shape)}")
+               lambda: f"position_ids must be [{B}, {S}], [1, {S}] or [{S}], got {list(_u(position_ids).shape)}")
         pos = pos.expand(B, S)
     yq, yk = ops.rotary_paged.rope_freq(a, b, f, pos, bool(interleaved), float(attention_scale))
     if packed:
@@ -1044,9 +1044,9 @@ def fused_partial_rotary_embedding(q, k=None, inv_freq=None, position_ids=None, 
 
 def _paged_caches(name, key_cache, value_cache):
     kc, vc = _u(key_cache), _u(value_cache)
-    _check(kc.dim() == 4 and vc.shape == kc.shape, name, "caches must be [num_blocks, kv_heads, block_size, head_dim] "
+    _check(kc.dim() == 4 and vc.shape == kc.shape, name, lambda: "caches must be [num_blocks, kv_heads, block_size, head_dim] "
            f"of one shape, got {list(kc.shape)} and {list(vc.shape)}")
-    _check(vc.dtype == kc.dtype, name, f"key cache is {kc.dtype}, value cache {vc.dtype}")
+    _check(vc.dtype == kc.dtype, name, lambda: f"key cache is {kc.dtype}, value cache {vc.dtype}")
     _check(kc.stride(3) == 1 and vc.stride() == kc.stride(), name, "caches need equal strides and a unit inner stride")
     _check(kc.shape[1] > 0 and kc.shape[2] > 0, name, "caches need at least one head and one place in a block")
     return kc, vc
@@ -1073,20 +1073,20 @@ def paged_rotary_append(qkv, key_cache, value_cache, block_tables, seq_lens, cu_
     kc, vc = _paged_caches(name, key_cache, value_cache)
     D, Hkv = kc.shape[3], kc.shape[1]
     _check(t.dtype in ops.rotary_paged.FLOATS and t.dtype == kc.dtype, name,
-           f"qkv and caches must share a floating type, got {t.dtype} and {kc.dtype}")
+           lambda: f"qkv and caches must share a floating type, got {t.dtype} and {kc.dtype}")
     _check(t.dim() == 2 and t.shape[1] % D == 0 and t.shape[1] // D >= 2 * Hkv, name,
-           f"qkv must be [T, (Hq + {2 * Hkv}) * {D}], got {list(t.shape)}")
+           lambda: f"qkv must be [T, (Hq + {2 * Hkv}) * {D}], got {list(t.shape)}")
     tables = _int32(name, 'block_tables', block_tables, (None, None))
     B = tables.shape[0]
     lens = _int32(name, 'seq_lens', seq_lens, (B,))
     cu = None if cu_seqlens_q is None else _int32(name, 'cu_seqlens_q', cu_seqlens_q, (B + 1,))
-    _check(cu is not None or t.shape[0] == B, name, f"{t.shape[0]} tokens for {B} sequences need cu_seqlens_q")
+    _check(cu is not None or t.shape[0] == B, name, lambda: f"{t.shape[0]} tokens for {B} sequences need cu_seqlens_q")
     _check(tables.shape[1] > 0 or B == 0, name, "block_tables has no columns")
     f = None if inv_freq is None else _frequencies(name, inv_freq, D, interleaved)
     bias = None
     if qkv_bias is not None:
         bias = _u(qkv_bias)
-        _check(bias.numel() == t.shape[1], name, f"qkv_bias must have {t.shape[1]} values, got {bias.numel()}")
+        _check(bias.numel() == t.shape[1], name, lambda: f"qkv_bias must have {t.shape[1]} values, got {bias.numel()}")
         bias = bias.reshape(-1).to(t.dtype).contiguous()
     off = _u(position_offset)
     if isinstance(off, torch.Tensor):
@@ -1094,9 +1094,7 @@ def paged_rotary_append(qkv, key_cache, value_cache, block_tables, seq_lens, cu_
         off = off.reshape(1).to(torch.int32)
     _same_device(name, t, key_cache=kc, value_cache=vc, block_tables=tables, seq_lens=lens, cu_seqlens_q=cu, inv_freq=f,
                  qkv_bias=bias, position_offset=off)
-    with torch.no_grad():
-        q = ops.rotary_paged.paged_append(t.detach(), kc, vc, tables, lens, cu, f, bool(interleaved),
-                                          float(attention_scale), bias, off)
+    q = ops.rotary_paged.paged_append(t, kc, vc, tables, lens, cu, f, bool(interleaved), float(attention_scale), bias, off)
     return _w(q), key_cache if isinstance(key_cache, Tensor) else _w(kc), \
         value_cache if isinstance(value_cache, Tensor) else _w(vc)
 
@@ -1122,17 +1120,17 @@ def shared_prefix_attention(query, key_cache, value_cache, block_tables, seq_len
     q = _u(query)
     kc, vc = _paged_caches(name, key_cache, value_cache)
     _check(q.dim() == 3 and q.shape[2] == kc.shape[3], name,
-           f"query must be [T, heads, {kc.shape[3]}], got {list(q.shape)}")
+           lambda: f"query must be [T, heads, {kc.shape[3]}], got {list(q.shape)}")
     _check(q.dtype in ops.rotary_paged.FLOATS and q.dtype == kc.dtype, name,
-           f"query and caches must share a floating type, got {q.dtype} and {kc.dtype}")
-    _check(q.shape[1] % kc.shape[1] == 0, name, f"{q.shape[1]} query heads do not divide over {kc.shape[1]} key heads")
+           lambda: f"query and caches must share a floating type, got {q.dtype} and {kc.dtype}")
+    _check(q.shape[1] % kc.shape[1] == 0, name, lambda: f"{q.shape[1]} query heads do not divide over {kc.shape[1]} key heads")
     tables = _int32(name, 'block_tables', block_tables, (None, None))
     B = tables.shape[0]
     lens = _int32(name, 'seq_lens', seq_lens, (B,))
     cu = None if cu_seqlens_q is None else _int32(name, 'cu_seqlens_q', cu_seqlens_q, (B + 1,))
-    _check(cu is not None or q.shape[0] == B, name, f"{q.shape[0]} queries for {B} sequences need cu_seqlens_q")
+    _check(cu is not None or q.shape[0] == B, name, lambda: f"{q.shape[0]} queries for {B} sequences need cu_seqlens_q")
     most = 1 if cu is None else (q.shape[0] if max_seqlen_q is None else int(max_seqlen_q))
-    _check(most >= 1 or q.shape[0] == 0, name, f"max_seqlen_q must be positive, got {max_seqlen_q}")
+    _check(most >= 1 or q.shape[0] == 0, name, lambda: f"max_seqlen_q must be positive, got {max_seqlen_q}")
     pt, pl = None, 0
     if prefix_blocks is not None:
         pt = _int32(name, 'prefix_blocks', prefix_blocks, (None,))
@@ -1144,16 +1142,15 @@ def shared_prefix_attention(query, key_cache, value_cache, block_tables, seq_len
             pl = pl.reshape(1).to(torch.int32)
         else:
             _check(0 <= int(pl) <= pt.numel() * kc.shape[2], name,
-                   f"prefix_len {pl} does not fit {pt.numel()} blocks of {kc.shape[2]}")
+                   lambda: f"prefix_len {pl} does not fit {pt.numel()} blocks of {kc.shape[2]}")
     else:
         _check(prefix_len is None or not isinstance(_u(prefix_len), torch.Tensor) and int(prefix_len) == 0, name,
                "prefix_len without prefix_blocks")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    _check(scale > 0 and math.isfinite(scale), name, f"scale must be positive and finite, got {scale}")
+    _check(scale > 0 and math.isfinite(scale), name, lambda: f"scale must be positive and finite, got {scale}")
     aligned = kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in kc.stride()[:3])
     _check(aligned or not ops.prefix_attn.supported(q, kc, vc), name, "caches need 16-byte aligned rows")
     _same_device(name, q, key_cache=kc, value_cache=vc, block_tables=tables, seq_lens=lens, cu_seqlens_q=cu,
                  prefix_blocks=pt, prefix_len=pl)
-    with torch.no_grad():
-        o, lse = ops.prefix_attn.attend(q.detach(), kc, vc, tables, lens, pt, pl, cu, most, scale, bool(return_lse))
+    o, lse = ops.prefix_attn.attend(q, kc, vc, tables, lens, pt, pl, cu, most, scale, bool(return_lse))
     return (_w(o), _w(lse)) if return_lse else _w(o)

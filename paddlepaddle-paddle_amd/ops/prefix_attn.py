@@ -94,7 +94,8 @@ def attend(q, key_cache, value_cache, tables, lens, ptable, plen, cu, most, scal
     nblk, Hkv, page, _ = key_cache.shape
     B = lens.shape[0]
     if not supported(q, key_cache, value_cache):
-        o, lse = composite(q, key_cache, value_cache, tables, lens, ptable, plen, cu, scale)
+        with torch.no_grad():
+            o, lse = composite(q, key_cache, value_cache, tables, lens, ptable, plen, cu, scale)
         return o, lse if want_lse else None
     out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=q.device) if want_lse else None

@@ -24,12 +24,8 @@ def _alignment(ts):
     """Elements (at most 8) that divide every address and every stride but the last of the tensors."""
     a = 8
     for t in ts:
-        if t is None or t.numel() == 0:
-            continue
-        a = math.gcd(a, t.data_ptr() // t.element_size())
-        for s, n in zip(t.stride()[:-1], t.shape[:-1]):
-            if n > 1:
-                a = math.gcd(a, s)
+        if t is not None and t.numel():
+            a = math.gcd(a, t.data_ptr() // t.element_size(), *(s for s, n in zip(t.stride()[:-1], t.shape) if n > 1))
     return a
 
 
@@ -58,11 +54,13 @@ def angles(pos, inv_freq, scale):
 
 def _launch(q, k, inv_freq, pos, interleaved, scale, sign):
     B, S, Hq, D = q.shape
-    if interleaved and _alignment((q, k)) % 2:
-        q, k = q.contiguous(), None if k is None else k.contiguous()
     q = q if q.stride(3) == 1 else q.contiguous()
     if k is not None and k.stride(3) != 1:
         k = k.contiguous()
+    a = _alignment((q, k))
+    if interleaved and a % 2:
+        q, k = q.contiguous(), None if k is None else k.contiguous()
+        a = _alignment((q, k))
     yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
     f = inv_freq.double().contiguous()
@@ -71,7 +69,7 @@ def _launch(q, k, inv_freq, pos, interleaved, scale, sign):
                                    None if k is None else _strides(k), B, S, Hq, 0 if k is None else k.shape[2], D,
                                    f.numel(), int(interleaved), N.ptr(f), scale, N.ptr(pos),
                                    0 if pos is None else pos.stride(0), 0 if pos is None else pos.stride(1),
-                                   int(pos is not None and pos.dtype == torch.int64), sign, _alignment((q, k)),
+                                   int(pos is not None and pos.dtype == torch.int64), sign, a,
                                    N.dtcode(q.dtype), N.stream()), 'rope_freq')
     return yq, yk
 
@@ -91,32 +89,32 @@ class _RopeFreq(torch.autograd.Function):
     def backward(ctx, dq, dk):
         inv_freq, pos = ctx.saved_tensors
         interleaved, scale, sign = ctx.how
+        turn = _RopeFreq.apply if torch.is_grad_enabled() else _launch
         gq = gk = None
         if dq is not None:
-            gq, gk = _RopeFreq.apply(dq, dk, inv_freq, pos, interleaved, scale, -sign)
+            gq, gk = turn(dq, dk, inv_freq, pos, interleaved, scale, -sign)
         elif dk is not None:
-            gk, _ = _RopeFreq.apply(dk, None, inv_freq, pos, interleaved, scale, -sign)
+            gk, _ = turn(dk, None, inv_freq, pos, interleaved, scale, -sign)
         return gq, gk, None, None, None, None, None
 
 
 def rope_freq(q, k, inv_freq, pos, interleaved, scale):
     """q [B, S, Hq, D], k [B, S, Hk, D] or None; inv_freq [pairs]; pos [B, S] integers or None (0 .. S - 1)."""
     if _hip(q):
-        return _RopeFreq.apply(q, k, inv_freq, pos, interleaved, float(scale), 1.0)
+        wanted = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+        return (_RopeFreq.apply if wanted else _launch)(q, k, inv_freq, pos, interleaved, float(scale), 1.0)
     p = torch.arange(q.shape[1], device=q.device)[None] if pos is None else pos
     cos, sin = angles(p, inv_freq, scale)
     return rotate(q, cos, sin, interleaved), None if k is None else rotate(k, cos, sin, interleaved)
 
 
-def paged_append(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interleaved, scale, bias=None, offset=0,
-                 cos_table=None, sin_table=None, compute_dtype=None):
+def paged_append(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interleaved, scale, bias=None, offset=0):
     """q rows of qkv [T, (Hq + 2 Hkv) D] turned and returned [T, Hq, D]; keys turned and values written into the
-    pages of sequence b at places lens[b], lens[b] + 1, ...; the angle's position is the place + offset.  Angles
-    from inv_freq, or from tables [B, positions, pairs]."""
+    pages of sequence b at places lens[b], lens[b] + 1, ...; the angle's position is the place + offset."""
     nblk, Hkv, page, D = key_cache.shape
     T, B = qkv.shape[0], lens.shape[0]
     Hq = qkv.shape[1] // D - 2 * Hkv
-    pairs = inv_freq.numel() if inv_freq is not None else (0 if cos_table is None else cos_table.shape[-1])
+    pairs = 0 if inv_freq is None else inv_freq.numel()
     if _hip(qkv):
         qkv = qkv if qkv.stride(1) == 1 else qkv.contiguous()
         a = _alignment((qkv, key_cache, value_cache, bias))
@@ -134,10 +132,16 @@ def paged_append(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interl
                 N.ptr(qkv), qkv.stride(0), N.ptr(bias), N.ptr(q), N.ptr(key_cache), N.ptr(value_cache),
                 _strides(key_cache), N.ptr(tables), tables.stride(0), tables.shape[1], nblk, page, N.ptr(lens), N.ptr(cu),
                 N.ptr(offset) if dev else None, 0 if dev else int(offset), T, B, Hq, Hkv, D, pairs, int(interleaved),
-                N.ptr(f), float(scale), N.ptr(cos_table), N.ptr(sin_table),
-                0 if cos_table is None else cos_table.stride(0), 0 if cos_table is None else cos_table.shape[1], a,
-                N.dtcode(qkv.dtype), N.stream()), 'paged_append')
+                N.ptr(f), float(scale), a, N.dtcode(qkv.dtype), N.stream()), 'paged_append')
         return q
+    with torch.no_grad():
+        return _append_composite(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interleaved, scale, bias, offset)
+
+
+def _append_composite(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interleaved, scale, bias, offset):
+    nblk, Hkv, page, D = key_cache.shape
+    T, B = qkv.shape[0], lens.shape[0]
+    Hq = qkv.shape[1] // D - 2 * Hkv
     x = qkv.reshape(T, Hq + 2 * Hkv, D)
     x = x.float() + bias.float().reshape(1, Hq + 2 * Hkv, D) if bias is not None else x
     c = torch.arange(B + 1) if cu is None else cu.long().cpu()
@@ -149,12 +153,8 @@ def paged_append(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interl
         place = int(lens[b]) + torch.arange(r1 - r0, device=qkv.device)
         rows = x[r0:r1]
         qk = rows[:, :Hq + Hkv].to(torch.float32)
-        if pairs:
-            if cos_table is not None:
-                cs, sn = cos_table[b, place].float(), sin_table[b, place].float()
-            else:
-                cs, sn = angles(place + int(offset), inv_freq, scale)
-            qk = rotate(qk, cs, sn, interleaved)
+        if inv_freq is not None:
+            qk = rotate(qk, *angles(place + int(offset), inv_freq, scale), interleaved)
         q[r0:r1] = qk[:, :Hq].to(q.dtype)
         col = torch.div(place, page, rounding_mode='floor')
         has = (place >= 0) & (col < tables.shape[1])

@@ -49,7 +49,8 @@ def sample(x, u, temperature, top_k, top_p, min_p):
     """x [rows, V]; u [rows]; the settings scalars or [rows] tensors.  Returns (probs fp32, ids int64), [rows, 1]."""
     rows, V = x.shape
     if not _hip(x):
-        return composite(x, u, temperature, top_k, top_p, min_p)
+        with torch.no_grad():
+            return composite(x, u, temperature, top_k, top_p, min_p)
     x = x if x.stride(1) == 1 else x.contiguous()
     u = (u if u.dtype in (torch.float32, torch.float64) else u.float()).contiguous()
     keep = []

@@ -174,8 +174,7 @@ def filtered_sampling(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
         raise ValueError(f"filtered_sampling: uniform is on {u.device}, x on {t.device}")
     settings = (setting(temperature, 'temperature'), setting(top_k, 'top_k', True), setting(top_p, 'top_p'),
                 setting(min_p, 'min_p'))
-    with torch.no_grad():
-        probs, ids = ops.sampling.sample(t.detach(), u.detach().reshape(-1), *settings)
+    probs, ids = ops.sampling.sample(t, u.reshape(-1), *settings)
     return _w(probs), _w(ids)
 
 
