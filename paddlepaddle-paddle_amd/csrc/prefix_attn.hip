@@ -22,6 +22,7 @@
 // of zeros and masked: what lies in a page's unused slots never reaches a product.
 #define PA_FA_PAIR_GROUP_DECL static __constant__
 #include "flash_attn_kernels.h"
+#include "paged.h"
 
 namespace pa {
 namespace pfx {
@@ -886,13 +887,8 @@ __global__ __launch_bounds__(256) void join_kernel(Args A, int nw) {
   int b;
   bool over = false;
   if (A.cu) {
-    int lo = -1, hi = A.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (A.cu[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    b = t < A.cu[A.B] ? lo : -1;
+    b = __builtin_amdgcn_readfirstlane(seq_of_token(A.cu, A.B, t));
+    if (b == A.B) b = -1;
     if (b >= 0) {
       int tok0, n;
       seq_rows(A, b, tok0, n);
@@ -905,21 +901,30 @@ __global__ __launch_bounds__(256) void join_kernel(Args A, int nw) {
   const int pl = b >= 0 ? prefix_len(A) : 0, ol = b >= 0 ? own_len(A, b) : 0;
   const int rp = range_keys(pl, A.nsp > 0 ? A.nsp : 1, nw), ro = range_keys(ol, A.nso > 0 ? A.nso : 1, nw);
   const int ap = A.nsp > 0 ? (pl + rp - 1) / rp : 0, ao = A.nso > 0 ? (ol + ro - 1) / ro : 0;
+  // the parts' statistics by lane, 64 at a time; then their sums, several loads in flight
+  auto slot = [&](int s) { return (s < ap ? s : A.nsp + s - ap) * rows + row; };
+  auto stats = [&](int s) { return s < ap + ao ? A.wml[slot(s)] : make_float2(-INFINITY, 0.f); };
   float M = -INFINITY;
-  for (int s = 0; s < ap + ao; ++s) M = fmaxf(M, A.wml[(s < ap ? s : A.nsp + s - ap) * rows + row].x);
+  for (int s = lane; s - lane < ap + ao; s += 64) M = fmaxf(M, stats(s).x);
+  M = wave_max(M);
   float L = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < ap + ao; ++s) {
-    const long long i = (s < ap ? s : A.nsp + s - ap) * rows + row;
-    const float2 x = A.wml[i];
-    const float f = part_weight(x, M);
-    L += x.y * f;
-    float a[E];
-    load_f<float, E>(A.wa + i * D + lane * E, a);
+  for (int s0 = 0; s0 < ap + ao; s0 += 64) {
+    const float2 x = stats(s0 + lane);
+    const float w = s0 + lane < ap + ao ? part_weight(x, M) : 0.f;
+    L += x.y * w;
+    const int n = min(64, ap + ao - s0);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
+      float a[E];
+      load_f<float, E>(A.wa + slot(s0 + j) * D + lane * E, a);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += a[e] * f;
+      for (int e = 0; e < E; ++e) o[e] += a[e] * f;
+    }
   }
+  L = wave_sum(L);
   if (over) L = NAN;
   const float k = inverse_sum(L);
 #pragma unroll

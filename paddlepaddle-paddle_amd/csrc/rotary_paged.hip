@@ -14,7 +14,7 @@
 // on their way before the angles (and the token's place in the pages: three dependent loads) are known; with that,
 // blocks of 2 to 4 tokens are slower (0.61 GB of queries and keys in bf16: 67 us with one token a block, 69 with 2 or 4;
 // 8340 tokens to pages of 16: 31, 35, 39 us).
-#include "common.h"
+#include "paged.h"
 
 namespace pa {
 namespace rot {
@@ -194,18 +194,6 @@ struct AppendArgs {
   float scale;
   const double* inv_freq;
 };
-
-// Largest b with cu[b] <= t: B behind the last sequence, -1 before the first.  By a whole wave, 64 borders a step.
-__device__ __forceinline__ int seq_of_token(const int* cu, int B, int t) {
-  int lo = 0, n = B + 1;  // cu[0 .. lo) are <= t, cu[lo + n ..) are not
-  while (n > 0) {
-    const int step = (n + 63) / 64, i = (int)(threadIdx.x & 63) * step + step - 1;  // (a step's last border)
-    const int full = __popcll(__ballot(i < n && cu[lo + i] <= t));
-    lo += full * step;
-    n = step > 1 ? min(step - 1, n - full * step) : 0;
-  }
-  return lo - 1;
-}
 
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs A) {
