@@ -512,3 +512,223 @@ def test_sampling_refusals(dev):
                 dict(min_p=u[None, :2])):
         with pytest.raises(ValueError):
             paddle.filtered_sampling(x, u, **bad)
+
+
+# ------------------------------------------------------------------------------------------ together
+class Step:
+    """A layer of attention between an embedding and logits, over a paged cache behind a shared prefix.  Everything
+    but the four operators is a lookup, so that runs can be compared bit by bit."""
+
+    def __init__(self, dev, dtype, prompts, steps, plen, hq=4, hkv=2, d=64, page=16, vocab=200):
+        g = torch.Generator().manual_seed(7)
+        total = [n + steps for n in prompts]
+        self.kc, self.vc, self.tables, self.common = (t.to(dev) for t in
+                                                      paged(g, total, page, hkv, d, dtype, spare=-(-plen // page)))
+        self.embed = torch.randn(vocab, (hq + 2 * hkv) * d, generator=g).to(dtype).to(dev)
+        self.pick = torch.randint(0, hq * d, (vocab,), generator=g).to(dev)     # logits: values of the output
+        self.u = torch.rand(steps, len(prompts), generator=g).to(dev)
+        self.f, self.scale, self.plen = frequencies(d // 4).to(dev), 1.07, plen
+        self.prompts = [torch.randint(0, vocab, (n,), generator=g).to(dev) for n in prompts]
+        self.top_k = torch.tensor([0, 5, 40][:len(prompts)], device=dev, dtype=torch.int32)
+
+    def append(self, tokens, lens, cu=None):
+        return IF.paged_rotary_append(self.embed[tokens], self.kc, self.vc, self.tables, lens, cu, self.f, True, self.scale,
+                                      position_offset=self.plen)[0]
+
+    def attend(self, q, lens, cu=None, most=None):
+        return IF.shared_prefix_attention(q, self.kc, self.vc, self.tables, lens, self.common, self.plen, cu, most)
+
+    def sample(self, out, u):
+        x = out._t.reshape(out.shape[0], -1)[:, self.pick] * 9
+        return x, *paddle.filtered_sampling(x, u, 0.7, self.top_k, 0.9, 0.01)
+
+    def prefill(self):
+        """The prompts' keys and values; each one's last token goes to the first step."""
+        n = torch.tensor([len(p) - 1 for p in self.prompts], dtype=torch.int32)
+        cu = torch.cat([torch.zeros(1, dtype=torch.int32), n.cumsum(0).int()]).to(self.kc.device)
+        none = torch.zeros(len(n), dtype=torch.int32, device=self.kc.device)
+        if int(cu[-1]):
+            self.append(torch.cat([p[:-1] for p in self.prompts]), none, cu)
+        return n.to(self.kc.device), torch.stack([p[-1] for p in self.prompts])
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('dtype', [BF, HF, FF])
+def test_decode_loop(dev, dtype):
+    """Prompts appended in one ragged call, then single tokens: every step against the definitions on what the caches
+    held before it, and the caches at the end against one call of the whole sequences."""
+    steps, prompts, plen = 4, [5, 1, 20], 33
+    s = Step(dev, dtype, prompts, steps, plen)
+    start = s.kc.clone(), s.vc.clone()
+    lens, tokens = s.prefill()
+    said = [list(p.cpu()) for p in s.prompts]
+    for i in range(steps):
+        old, f = (s.kc.cpu(), s.vc.cpu()), s.f.cpu()
+        q = s.append(tokens, lens)
+        wq, wk, wv = O.append(s.embed[tokens].cpu(), *old, s.tables.cpu(), lens.cpu(), None, f, True, s.scale, plen)
+        half = torch.finfo(dtype).eps / 2
+        near(q._t, wq, wq.abs() * half + 1e-5)
+        near(s.kc, wk, wk.abs() * half + 1e-5)
+        assert torch.equal(s.vc.cpu().double(), wv)
+        lens = lens + 1
+        out = s.attend(q, lens)
+        want, _, size = O.attention(q._t.cpu(), s.kc.cpu(), s.vc.cpu(), s.tables.cpu(), lens.cpu(), s.common.cpu(), plen, None,
+                                    1 / math.sqrt(q.shape[2]))
+        near(out._t, want, O.attention_bound(want, size, dtype))
+        x, probs, ids = s.sample(out, s.u[i])
+        for b in range(len(prompts)):
+            token, share = O.sample(x[b].cpu(), float(s.u[i, b]), 0.7, int(s.top_k[b]), 0.9, 0.01)
+            assert int(ids._t[b, 0]) == token
+            assert abs(float(probs._t[b, 0]) - share) <= share * 2 ** -23 + 1e-9
+            said[b].append(ids._t[b, 0].cpu())
+        tokens = ids._t[:, 0]
+    whole = Step(dev, dtype, prompts, steps, plen)
+    whole.kc.copy_(start[0]), whole.vc.copy_(start[1])
+    n = torch.tensor([len(t) - 1 for t in said], dtype=torch.int32)
+    whole.append(torch.cat([torch.stack(t[:-1]) for t in said]).to(dev), torch.zeros_like(n).to(dev),
+                 torch.cat([torch.zeros(1, dtype=torch.int32), n.cumsum(0).int()]).to(dev))
+    assert torch.equal(whole.kc, s.kc) and torch.equal(whole.vc, s.vc)
+
+
+def run_steps(s, lens, tokens, replay=None):
+    """Steps one after the other, in place on (lens, tokens, u): what is said, and the last outputs."""
+    said = []
+    u = s.u[0].clone()
+
+    def step():
+        q = s.append(tokens, lens)
+        lens.add_(1)
+        out = s.attend(q, lens)
+        _, probs, ids = s.sample(out, u)
+        tokens.copy_(ids._t[:, 0])
+        return out._t, probs._t
+    if replay is not None:
+        replay(step)
+    for i in range(s.u.shape[0]):
+        u.copy_(s.u[i])
+        outs = step() if replay is None else replay(None)
+        said.append((tokens.clone(), outs[0].clone(), outs[1].clone()))
+    return said
+
+
+class Captured:
+    def __init__(self, s, lens, tokens):
+        self.keep = (s, lens, tokens)
+
+    def __call__(self, step):
+        if step is not None:
+            s, lens, tokens = self.keep
+            was = s.kc.clone(), s.vc.clone(), lens.clone(), tokens.clone()
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.current_stream().wait_stream(side)
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph):
+                self.outs = step()
+            for t, v in zip((s.kc, s.vc, lens, tokens), was):   # (the step that warmed up)
+                t.copy_(v)
+            return None
+        self.graph.replay()
+        return self.outs
+
+
+@pytest.mark.gpu
+def test_captured_steps_replay():
+    """Steps replayed from a graph, with eager steps of another batch and synchronizations between, give what eager
+    steps give; two graphs and an eager batch at once on three streams as well."""
+    def fresh():
+        s = Step('cuda', BF, [5, 1, 20], 6, 40)
+        return s, *s.prefill()
+    want = run_steps(*fresh())
+
+    def same(got):
+        for w, g in zip(want, got, strict=True):
+            for a, b in zip(w, g):
+                assert torch.equal(a, b)
+    same(run_steps(*fresh()))                                   # the same again, bit by bit
+    s, lens, tokens = fresh()
+    cap = Captured(s, lens, tokens)
+
+    def between(step):
+        if step is None:
+            same(run_steps(*fresh()))
+            torch.cuda.synchronize()
+        return cap(step)
+    same(run_steps(s, lens, tokens, between))
+    torch.cuda.synchronize()
+    # at once
+    runs = []
+    for k in range(3):
+        s, lens, tokens = fresh()
+        u, got = s.u[0].clone(), []
+        cap = Captured(s, lens, tokens) if k < 2 else None
+
+        def step(s=s, lens=lens, tokens=tokens, u=u):
+            q = s.append(tokens, lens)
+            lens.add_(1)
+            out = s.attend(q, lens)
+            _, probs, ids = s.sample(out, u)
+            tokens.copy_(ids._t[:, 0])
+            return out._t, probs._t
+        if cap is not None:
+            cap(step)
+        runs.append((s, tokens, u, got, (lambda cap=cap: cap(None)) if cap is not None else step, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for s, tokens, u, got, go, stream in runs:
+            with torch.cuda.stream(stream):
+                u.copy_(s.u[i])
+                outs = go()
+                got.append((tokens.clone(), outs[0].clone(), outs[1].clone()))
+    torch.cuda.synchronize()
+    for r in runs:
+        same(r[3])
+
+
+@pytest.mark.gpu
+def test_rotary_captured_both_ways():
+    """Forward and backward in one graph, of leaves that no eager graph holds, replayed between eager calls."""
+    g = torch.Generator().manual_seed(5)
+    mk = lambda: torch.randn(2, 65, 6, 64, generator=g).to(BF).cuda()  # noqa: E731
+    f = frequencies(16).cuda()
+    x, dy = mk().requires_grad_(), mk()
+
+    def both(x, dy):
+        q, k = IF.fused_partial_rotary_embedding(x[:, :, :4], x[:, :, 4:], f)
+        return torch.cat([q._t.detach(), k._t.detach()], 2), torch.autograd.grad([q._t, k._t], x, [dy[:, :, :4], dy[:, :, 4:]])[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(x, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both(x, dy)
+    for _ in range(4):
+        a, b = mk(), mk()
+        with torch.no_grad():
+            x.copy_(a), dy.copy_(b)
+        graph.replay()
+        want = both(a.requires_grad_(), b)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_answers_do_not_change_between_calls():
+    """Sums by atomics are of integers, joins have one order."""
+    g = torch.Generator().manual_seed(6)
+    x = (torch.randn(9, 60000, generator=g) * 2).to(BF).cuda()
+    u = torch.rand(9, generator=g).cuda()
+    kc, vc, tables, common = paged(g, [70, 300, 5] * 8, 16, 2, 128, BF, spare=80)
+    q = torch.randn(24, 16, 128, generator=g).to(BF).cuda()
+    lens = torch.tensor([70, 300, 5] * 8, dtype=torch.int32).cuda()
+    args = q, kc.cuda(), vc.cuda(), tables.cuda(), lens, common.cuda(), 1270
+    first = None
+    for _ in range(5):
+        got = [t._t for t in (*paddle.filtered_sampling(x, u, 0.9, 0, 0.95), *paddle.filtered_sampling(x, u, 1.5, 3000, 0.9, 1e-4),
+                              *IF.shared_prefix_attention(*args, return_lse=True))]
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
