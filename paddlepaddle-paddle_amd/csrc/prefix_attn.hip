@@ -1001,14 +1001,15 @@ PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, i
   return 0;
 }
 
+// ws: plan[4] * T * Hq * (D + 2) floats, partial outputs and their (max, sum)
 PA_API int pa_prefix_attn(const void* q, const void* kc, const void* vc, long long qt, long long qh,
                           const long long* cstr, const int* tables, long long tstride, int max_blocks,
                           const int* ptable, int pblocks, const int* plen_dev, int plen, int num_blocks, int page,
-                          const int* lens, const int* cu, void* out, float* lse, float* wa, float* wml,
+                          const int* lens, const int* cu, void* out, float* lse, float* ws,
                           const int* plan, int T, int B, int Hq, int Hkv, int D, int most, float scale, int dt,
                           hipStream_t st) {
   if (T <= 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || page <= 0 || num_blocks < 0 || (dt != 1 && dt != 2) ||
-      !(scale > 0.f) || cstr[2] > (1 << 27) || (!cu && T != B) || (plan[4] > 0 && (!wa || !wml)))
+      !(scale > 0.f) || cstr[2] > (1 << 27) || (!cu && T != B) || (plan[4] > 0 && !ws))
     return (int)hipErrorInvalidValue;
   Args A;
   A.q = (const uint16_t*)q; A.kc = (const uint16_t*)kc; A.vc = (const uint16_t*)vc;
@@ -1016,7 +1017,7 @@ PA_API int pa_prefix_attn(const void* q, const void* kc, const void* vc, long lo
   A.tables = tables; A.tstride = tstride; A.max_blocks = max_blocks;
   A.ptable = ptable; A.pblocks = pblocks; A.plen_dev = plen_dev; A.plen = plen;
   A.lens = lens; A.cu = cu;
-  A.out = (uint16_t*)out; A.lse = lse; A.wa = plan[4] > 0 ? wa : nullptr; A.wml = (float2*)wml; A.most = most;
+  A.out = (uint16_t*)out; A.lse = lse; A.wa = plan[4] > 0 ? ws : nullptr; A.wml = (float2*)(ws + (long long)plan[4] * T * Hq * D); A.most = most;
   A.num_blocks = num_blocks; A.page = page;
   A.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
   A.T = T; A.B = B; A.Hq = Hq; A.Hkv = Hkv; A.G = Hq / Hkv;

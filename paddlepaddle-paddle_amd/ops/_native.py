@@ -173,7 +173,7 @@ _SIGS = {
     'pa_rope_freq': [P, P, P, P, LLP, LLP, I, I, I, I, I, I, I, P, F, P, LL, LL, I, F, I, I, P],
     'pa_paged_append': [P, LL, P, P, P, P, LLP, P, LL, I, I, I, P, P, P, LL, I, I, I, I, I, I, I, P, F, I, I, P],
     'pa_prefix_attn_plan': [I, I, I, I, I, I, I, LL, LL, IP],
-    'pa_prefix_attn': [P, P, P, LL, LL, LLP, P, LL, I, P, I, P, I, I, I, P, P, P, P, P, P, IP, I, I, I, I, I, I, F, I, P],
+    'pa_prefix_attn': [P, P, P, LL, LL, LLP, P, LL, I, P, I, P, I, I, I, P, P, P, P, P, IP, I, I, I, I, I, I, F, I, P],
     'pa_sample_ws_bytes': [I],
     'pa_sample': [P, LL, I, I, P, I, P, P, P, P, D, I, D, D, P, P, P, I, P],
     'pa_flash_fwd': [P, P, P, P, P, I, I, I, I, I, I, LLP, LLP, LLP, LLP, F, I, I, P],
@@ -219,7 +219,8 @@ def check(err, name):
 
 
 def stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (torch.cuda.current_stream() makes a Stream object each time: 4 us of a launch's 20)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def device_of(t):
@@ -236,7 +237,7 @@ def ptr(t):
         return None
     if t.device.type != 'cuda':
         raise RuntimeError(f"HIP kernel operand on {t.device} (expected a GPU tensor)")
-    return ctypes.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def dtcode(dt):

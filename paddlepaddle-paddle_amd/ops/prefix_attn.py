@@ -110,16 +110,13 @@ def attend(q, key_cache, value_cache, tables, lens, ptable, plen, cu, most, scal
     most = max(1, min(most, T))
     N.check(N.lib.pa_prefix_attn_plan(T, B, Hq, Hkv, D, most, int(cu is not None), cap if dev else min(int(plen), cap),
                                       tables.shape[1] * page, plan), 'prefix_attn_plan')
-    wa = wml = None
-    if plan[4]:
-        # this call's own workspace: two streams or two captured graphs never share one
-        wa = torch.empty(plan[4] * T * Hq * D, dtype=torch.float32, device=q.device)
-        wml = torch.empty(plan[4] * T * Hq * 2, dtype=torch.float32, device=q.device)
+    # this call's own workspace: two streams or two captured graphs never share one
+    ws = torch.empty(plan[4] * T * Hq * (D + 2), dtype=torch.float32, device=q.device) if plan[4] else None
     with N.device_of(q):
         N.check(N.lib.pa_prefix_attn(
             N.ptr(q), N.ptr(key_cache), N.ptr(value_cache), q.stride(0), q.stride(1),
             (ctypes.c_longlong * 3)(*key_cache.stride()[:3]), N.ptr(tables), tables.stride(0), tables.shape[1],
             N.ptr(ptable), 0 if ptable is None else ptable.numel(), N.ptr(plen) if dev else None,
-            0 if dev else min(int(plen), cap), nblk, page, N.ptr(lens), N.ptr(cu), N.ptr(out), N.ptr(lse), N.ptr(wa),
-            N.ptr(wml), plan, T, B, Hq, Hkv, D, most, float(scale), N.dtcode(q.dtype), N.stream()), 'prefix_attn')
+            0 if dev else min(int(plen), cap), nblk, page, N.ptr(lens), N.ptr(cu), N.ptr(out), N.ptr(lse), N.ptr(ws),
+            plan, T, B, Hq, Hkv, D, most, float(scale), N.dtcode(q.dtype), N.stream()), 'prefix_attn')
     return out, lse
