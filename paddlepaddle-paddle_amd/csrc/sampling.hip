@@ -410,6 +410,21 @@ constexpr double kFix = 562949953421312.0;
 __device__ __forceinline__ unsigned long long fixed(double w) {
   return __builtin_bit_cast(unsigned long long, fma(w, kFix, 4503599627370496.0)) & 0xfffffffffffffull;
 }
+// The least key whose logit's bin is b or before it.  By a whole wave, 6 bits a step.
+__device__ __forceinline__ uint32_t least_key(const Grid& G, int b) {
+  const uint32_t lane = threadIdx.x & 63, top = key_of(INFINITY);
+  uint32_t key = 0;  // (0: no token's)
+#pragma unroll 1
+  for (int sh = 26; sh >= -4; sh -= 6) {
+    const uint32_t step = sh >= 0 ? lane << sh : lane >> 4, k = key + step;  // (the last step: its 4 keys, 16 times each)
+    const float v = value_of(k);
+    const bool in = k >= top || (v > -INFINITY && G.bin(v) <= b);
+    const int before = __popcll(__ballot(!in));
+    if (before == 0) break;
+    key += sh >= 0 ? (uint32_t)(before - 1) << sh : (uint32_t)before >> 4;
+  }
+  return key;
+}
 // a token's place in the order: larger ones come first
 __device__ __forceinline__ unsigned long long place(uint32_t key, uint32_t i) {
   return (unsigned long long)key << 32 | (0xffffffffu - i);
@@ -417,19 +432,18 @@ __device__ __forceinline__ unsigned long long place(uint32_t key, uint32_t i) {
 
 // E consecutive tokens from i on; -inf past the end
 template <typename T, int E>
-__device__ __forceinline__ void load_tokens(const T* __restrict__ x, int i, int end, bool vec, float (&o)[E]) {
+__device__ __forceinline__ void load_tokens(const T* __restrict__ x, int i, int end, bool vec, T (&o)[E]) {
   if (vec && i + E <= end) {
     constexpr int W = 16 / sizeof(T) < E ? 16 / sizeof(T) : E;
 #pragma unroll
     for (int j = 0; j < E; j += W) {
-      float v[W];
-      load_f<T, W>(x + i + j, v);
+      const Pack<T, W> v = *reinterpret_cast<const Pack<T, W>*>(x + i + j);
 #pragma unroll
-      for (int e = 0; e < W; ++e) o[j + e] = v[e];
+      for (int e = 0; e < W; ++e) o[j + e] = v.v[e];
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < E; ++j) o[j] = i + j < end ? to_f(x[i + j]) : -INFINITY;
+    for (int j = 0; j < E; ++j) o[j] = i + j < end ? x[i + j] : from_f<T>(-INFINITY);
   }
 }
 template <typename T>
@@ -457,7 +471,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
   }
   constexpr int E = 8, P = CH / (256 * E);  // a thread's tokens: P times E in a row, a wave's: P parts
   static_assert(SUB == 64 * E, "a part is a wave's");
-  float v[P][E];
+  T v[P][E];
   const bool vec = vector_rows<T>(A);
   uint32_t valid = 0;
 #pragma unroll
@@ -468,7 +482,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const uint32_t k = key_of(v[j][e]);
+      const uint32_t k = key_of(to_f(v[j][e]));
       valid += k != 0;
       m = max(m, k);
     }
@@ -488,7 +502,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
     if (rk[j * 4 + wave] == mk && mk != 0) {  // the part has it
 #pragma unroll
       for (int e = E - 1; e >= 0; --e)
-        if (key_of(v[j][e]) == mk) atomicMin(&ri, (uint32_t)(i0 + (j * 256 + tid) * E + e));
+        if (key_of(to_f(v[j][e])) == mk) atomicMin(&ri, (uint32_t)(i0 + (j * 256 + tid) * E + e));
     }
   __syncthreads();
   if (tid == 0) {
@@ -503,13 +517,13 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
   // what takes longest
 #pragma unroll 1
   for (int j = 0; j < P; ++j) {
-    float q[E];
+    T q[E];
     load_tokens<T, E>(x, i0 + (j * 256 + tid) * E, end, vec, q);
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (key_of(q[e]) != 0) {
+      if (key_of(to_f(q[e])) != 0) {
         double f;
-        const int b = G.bin(q[e], f);
+        const int b = G.bin(to_f(q[e]), f);
         atomicAdd(&count[b], 1u);
         atomicAdd(&mass[b], part_mass(f));
       }
@@ -538,14 +552,20 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   __shared__ uint32_t ln;                     // their number
   __shared__ uint32_t pcount[256];
   __shared__ unsigned long long pmass[256], fsh;
-  __shared__ double red[NW];
+  __shared__ double red[NW], scale[NB];
   __shared__ uint32_t kmax, kmin;             // their keys
   __shared__ int bsh, shift[MC], with[WITH], wn;
   __shared__ unsigned long long got[2];
 
-  const Setting S = setting(A, r);
   uint32_t mk = 0, mi = 0xffffffffu, valid = 0;
-  for (int c = tid; c < nc; c += NT) {
+  if (tid < nc) {
+    mk = C[tid].key;
+    mi = C[tid].first;
+    valid = C[tid].valid;
+  }
+  const uint32_t own_key = mk;
+  const Setting S = setting(A, r);
+  for (int c = tid + NT; c < nc; c += NT) {
     const uint32_t k = C[c].key, i = C[c].first;
     valid += C[c].valid;
     if (k > mk || (k == mk && i < mi)) {
@@ -587,12 +607,12 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   auto shifts = [&](int c0) {
     __syncthreads();
     if (tid < MC && c0 + tid < nc) {
-      const uint32_t k = C[c0 + tid].key;
+      const uint32_t k = c0 ? C[c0 + tid].key : own_key;
       shift[tid] = k ? G.bin(value_of(k)) : NB;
     }
     __syncthreads();
   };
-  const double bin_scale = exp2_64(-0.125 * (double)(tid + 1)) * (1.0 / kPart);  // of bin tid
+  if (tid < NB) scale[tid] = exp2_64(-0.125 * (double)(tid + 1)) * (1.0 / kPart);  // of a bin's mass
 
   // the chunks' histograms, joined; the last bin has no mass
   {
@@ -602,7 +622,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
       shifts(c0);
       if (tid < NB - 1) {
         const int e = min(MC, nc - c0);
-#pragma unroll 8
+#pragma unroll 16
         for (int c = 0; c < e; ++c) {
           const int b = tid - shift[c], at = max(b, 0);
           const uint32_t cn = C[c0 + c].count[at];
@@ -614,7 +634,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     }
     if (tid < NB) {
       cum[tid] = n;
-      cmass[tid] = w * bin_scale;
+      cmass[tid] = w * scale[tid];
     }
   }
   __syncthreads();
@@ -646,6 +666,8 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     if (cum[b1] - (b0 ? cum[b0 - 1] : 0u) > CAP) return false;
     listed = b1;
     constexpr int PP = CH / SUB;
+    // their logits: [from, upto)
+    const float from = value_of(least_key(G, b1)), upto = b0 ? value_of(least_key(G, b0 - 1)) : INFINITY;
     __syncthreads();  // the list before has been read
     if (tid == 0) {
       ln = 0;
@@ -657,48 +679,52 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
       __syncthreads();
       for (int p = p0 + tid; p < min(p0 + WITH, nc * PP); p += NT) {
         const uint32_t k = C[p / PP].part[p % PP];
-        if (k != 0 && G.bin(value_of(k)) <= b1) with[atomicAdd(&wn, 1)] = p;
+        if (k != 0 && value_of(k) >= from) with[atomicAdd(&wn, 1)] = p;
       }
       __syncthreads();
       const int n = wn;
-      auto fetch = [&](int j, float (&v)[8]) {
-        const int i = j < n ? with[j] * SUB : A.V;
-        load_tokens<T, 8>(x, i + lane * 8, j < n ? min(A.V, i + SUB) : 0, vec, v);
-      };
-      float next[8];
-      fetch(wave, next);
+      // PF parts of a wave are on their way at once: as many bytes as its registers take
+      constexpr int PF = sizeof(T) == 2 ? 4 : 2;
 #pragma unroll 1
-      for (int j = wave; j < n; j += NW) {
-        float v[8];
+      for (int g = wave; g < n; g += PF * NW) {
+        T raw[PF][8];
+        int first[PF];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = next[e];
-        fetch(j + NW, next);
-        const int i = with[j] * SUB + lane * 8;
-        uint32_t hit = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int b = G.bin(v[e]);
-          if (b >= b0 && b <= b1 && key_of(v[e]) != 0) hit |= 1u << e;
+        for (int k = 0; k < PF; ++k) {
+          const int j = g + k * NW;
+          first[k] = j < n ? with[j] * SUB + lane * 8 : A.V;
+          load_tokens<T, 8>(x, first[k], A.V, vec, raw[k]);
         }
-        if (__ballot(hit != 0) == 0) continue;
-        // the wave's tokens one behind the other
-        const uint32_t n_ = __popc(hit), upto = wave_scan(n_), all = lane_value(upto, 63);
-        uint32_t at = 0;
-        if (lane == 0) at = atomicAdd(&ln, all);
-        at = lane_value(at, 0) + upto - n_;
+        auto in = [&](int k, int e) {
+          const float v = to_f(raw[k][e]);
+          return v >= from && (b0 == 0 || v < upto);
+        };
+        int own = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (hit >> e & 1) {
-            if (at < CAP) list[at].place = place(key_of(v[e]), i + e);
-            ++at;
-          }
+        for (int k = 0; k < PF; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) own += in(k, e);
+        const int before = wave_scan(own), all = lane_value(before, 63);
+        if (all == 0) continue;
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&ln, (uint32_t)all);
+        at = lane_value(at, 0) + before - own;
+#pragma unroll
+        for (int k = 0; k < PF; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (in(k, e)) {
+              if (at < CAP) list[at].place = first[k] + e;
+              ++at;
+            }
       }
       __syncthreads();
     }
+    if (ln > CAP) return false;
     uint32_t hi = 0, lo = 0xffffffffu;
     for (uint32_t i = tid; i < ln; i += NT) {
-      const uint32_t k = (uint32_t)(list[i].place >> 32);
-      list[i].w = fixed(G.weight(value_of(k)));
+      const uint32_t id = (uint32_t)list[i].place, k = key_of(to_f(x[id]));
+      list[i] = Token{place(k, id), fixed(G.weight(value_of(k)))};
       hi = max(hi, k);
       lo = min(lo, k);
     }
@@ -771,8 +797,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
       width = min(width - ((unsigned long long)q << sh), (1ull << sh) - 1);
       __syncthreads();
     }
-    // The window's tokens, at most 64 (places are all different), ranked by one wave: those within the cut are the
-    // first in the order, and the last of them has one less before it than they are.
+    // The window's tokens, at most 64 (places are all different), each ranked by 8 lanes
     if (n > 64) {
       if (tid == 0) pcount[0] = 0;
       __syncthreads();
@@ -786,22 +811,34 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
         }
       __syncthreads();
     }
-    if (wave == 0) {
+    {
+      static_assert(NT == 64 * 8, "a token takes 8 lanes");
       const uint32_t np = n > 64 ? min(pcount[0], 64u) : n;
-      Token t{0, 0};
-      if ((uint32_t)lane < np) t = n > 64 ? Token{pmass[lane], pmass[64 + lane]} : list[lane];
-      const bool have = t.w != 0;
+      auto token = [&](uint32_t i) {
+        return i >= np ? Token{0, 0} : (n > 64 ? Token{pmass[i], pmass[64 + i]} : list[i]);
+      };
+      const Token t = token(tid >> 3);
       const unsigned long long mine = order(t);
-      uint32_t rank = 0;
-      unsigned long long m = w0;
-      for (uint32_t j = 0; j < np; ++j) {
-        const unsigned long long w = lane_value(t.w, j);
-        const bool first = w != 0 && lane_value(mine, j) > mine;
-        rank += first;
-        m += first ? w : 0ull;
+      uint32_t c = 0;  // the window's kept tokens before this one, and (<< 16) all of them
+      unsigned long long m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const Token o = token(8 * j + (tid & 7));
+        const bool before = o.w != 0 && order(o) > mine;
+        c += (o.w != 0 ? 0x10000u : 0u) + before;
+        m += before ? o.w : 0ull;
       }
-      const unsigned long long ok = __ballot(have && (by_mass ? m < room || n0 + rank == 0 : n0 + rank <= last));
-      if (have && rank + 1 == (uint32_t)__popcll(ok)) {
+      c += from_lane<0xb1, 0xf>(c);  // the neighbour's, the neighbour pair's, the other four's (mirrored)
+      m += from_lane<0xb1, 0xf>(m);
+      c += from_lane<0x4e, 0xf>(c);
+      m += from_lane<0x4e, 0xf>(m);
+      c += from_lane<0x141, 0xf>(c);
+      m += from_lane<0x141, 0xf>(m);
+      const uint32_t rank = n0 + (c & 0xffff);
+      const bool end = (c & 0xffff) + 1 == c >> 16;  // the window's last
+      m += w0;
+      const bool cut = by_mass ? (m < room || rank == 0) && (m + t.w >= room || end) : rank == last || (rank < last && end);
+      if (t.w != 0 && cut && (tid & 7) == 0) {
         got[0] = t.place;
         got[1] = m + t.w;
       }
@@ -912,14 +949,12 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
   }
   auto passes = [&](unsigned long long at, double w) { return at >= tp && w >= least; };
   const double part = partial ? (double)keep(tp) * (1.0 / kFix) : 0.0;
-  const double total = (bf > 0 ? cmass[bf - 1] : 0.0) + part, goal = S.u * total;
+  const double total = (bf > 0 ? cmass[bf - 1] : 0.0) + part;
+  const double goal = S.u * total * (1.0 + 0x1p-40);  // a mass that meets it exactly does not pass it
 
   // the chunk in which the kept mass passes the goal: a wave sums a chunk's whole bins and its listed tokens
   double run = 0.0, start = 0.0, lastrun = 0.0;
   int at = -1, lastc = -1;
-  double scale[NB / 64];  // of this lane's bins of a chunk, before its shift
-#pragma unroll
-  for (int j = 0; j < NB / 64; ++j) scale[j] = exp2_64(-0.125 * (double)(lane + 64 * j + 1)) * (1.0 / kPart);
   for (int c0 = 0; c0 < nc && at < 0; c0 += NW) {
     if (nc > MC && c0 % MC == 0) shifts(c0);
     const int c = c0 + wave;
@@ -929,7 +964,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
 #pragma unroll
       for (int j = 0; j < NB / 64; ++j) {
         const int b = lane + 64 * j;
-        w += b < hi ? (double)C[c].mass[b] * scale[j] : 0.0;
+        w += b < hi ? (double)C[c].mass[b] * scale[b] : 0.0;
       }
       w *= exp2_64(-0.125 * (double)shift[c % MC]);
       if (partial) {
@@ -961,8 +996,9 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     at = lastc;
     start = lastrun;
   }
-  // Scan of that chunk: the waves' parts, then the part in which the goal is passed, 64 tokens at a time
-  const int i0 = at * CH + wave * (CH / NW), i1 = min(A.V, i0 + CH / NW);
+  // Scan of that chunk: the waves' parts, then the lanes of the part in which the goal is passed, then one lane's tokens
+  constexpr int E = CH / NT;
+  const int i0 = at * CH + tid * E, i1 = min(A.V, at * CH + CH);
   auto mass_of = [&](int i, float q) -> double {
     const uint32_t k = key_of(q);
     const int b = k != 0 ? G.bin(q) : NB;
@@ -970,19 +1006,17 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     const double w = G.weight(q);
     return b < bf || passes(place(k, i), w) ? w : 0.0;
   };
-  auto token = [&](int i) { return i < i1 ? to_f(x[i]) : -INFINITY; };
-  double sum = 0.0;
-#pragma unroll 1
-  for (int i = i0 + lane; i - lane < i1; i += 256) {
-    float q[4];
+  double each[E], sum = 0.0;
+  {
+    T q[E];
+    load_tokens<T, E>(x, i0, i1, vec, q);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = token(i + 64 * j);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum += mass_of(i + 64 * j, q[j]);
+    for (int e = 0; e < E; ++e) sum += each[e] = mass_of(i0 + e, to_f(q[e]));
   }
-  sum = wave_add(sum);
+  const double before = wave_scan(sum) - sum;
+  const double all = wave_add(sum);
   __syncthreads();
-  if (lane == 0) red[wave] = sum;
+  if (lane == 0) red[wave] = all;
   __syncthreads();
   int mine = -1;
   double from = 0.0, upto = start;
@@ -996,27 +1030,22 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     upto = next;
   }
   if (wave != mine) return;
-  int found = i0;
-  double share = 0.0;
-  float next = token(i0 + lane);
-#pragma unroll 1
-  for (int i = i0; i < i1; i += 64) {
-    const float q = next;
-    next = token(i + 64 + lane);
-    const double w = mass_of(i + lane, q), c = wave_scan(w);
-    const unsigned long long any = __ballot(w > 0.0), hit = __ballot(w > 0.0 && from + c > goal);
-    if (any) {
-      const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any);  // (rounding: the last with mass)
-      found = i + l;
-      share = lane_value(w, l);
-      if (hit) break;
+  const unsigned long long any = __ballot(sum > 0.0), hit = __ballot(sum > 0.0 && from + before + sum > goal);
+  if (lane != (hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any))) return;  // (rounding: the last that has any)
+  int found = 0;
+  double mass = 0.0, run_ = from + before;
+  bool past = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    run_ += each[e];
+    if (each[e] > 0.0 && !past) {
+      found = i0 + e;
+      mass = each[e];
+      past = run_ > goal;
     }
-    from += lane_value(c, 63);
   }
-  if (lane == 0) {
-    A.ids[r] = found;
-    A.probs[r] = (float)(share / total);
-  }
+  A.ids[r] = found;
+  A.probs[r] = (float)(mass / total);
 }
 
 }  // namespace smp
