@@ -189,6 +189,9 @@ constexpr int lds_bytes() {
   return (stage > join ? stage : join) + NW * RT * 16 * 8 + RT * 16 * D;
 }
 
+// What bounds it: the read of its keys and values where rows are few (own pages of 256 sequences of 500 .. 1500 keys,
+// 8 heads of 128: 218 us, 4.85 TB/s); the launch and three dependent loads for a small call (4 sequences of 32 heads
+// behind 1000 keys: 10 us, and 4 for the join).
 // One item: rows [row0, row0 + 16 RT) of `nrows` rows (row r = token tok0 + r / G, head hk G + r % G)
 // against keys [k0, k1) of `table`; row r sees keys < lim0 + r / G (CAUSAL) or all.
 template <typename T, int D, int RT, int NW, bool CAUSAL>
@@ -515,7 +518,10 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
 // A prefix item of many rows: the NW waves share each tile of 64 keys, two of which are in LDS, and have 16 RT
 // rows of their own: rows [row0, row0 + 16 RT NW) against keys [k0, k1), all of which every row sees.  In the
 // layout of item() each wave reads all of its own keys from L2, 32 rows at a time: at 2048 rows a key head that
-// is 19 TB/s of L2 reads, which bound it (518 TFLOP/s); here a tile serves 8 times as many rows.
+// is 19 TB/s of L2 reads, which bound it (518 TFLOP/s); here a tile serves 8 times as many rows (860 TFLOP/s for 256
+// queries of 64 heads behind 32768 keys of 8 heads, 128 values each).  What bounds it now: no one thing; without the
+// DMA, the barrier, the exponentials, the value product or the LDS reads alone it takes 84 to 94 % of its time, and 256
+// registers leave two waves a SIMD to cover each other's waits.
 constexpr int kWideRT = 2;
 // Tiles between two meetings of a block's waves: what LDS holds in rings of twice as many
 template <int D>
@@ -828,7 +834,7 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
 __device__ __forceinline__ void seq_rows(const Args& A, int b, int& tok0, int& n) {
   tok0 = A.cu ? A.cu[b] : b;
   n = A.cu ? A.cu[b + 1] - tok0 : 1;
-  if (tok0 < 0 || n < 0 || tok0 + n > A.T || n > A.most) n = 0;  // offsets that do not fit the call: nothing is read
+  if (tok0 < 0 || tok0 > A.T || n < 0 || n > A.most || tok0 + n > A.T) n = 0;  // offsets that do not fit the call: nothing is read
 }
 
 // Items in the order of dispatch, 8 blocks at a time (one per XCD): the prefix items, which take longest, then the
@@ -875,7 +881,8 @@ __global__ __launch_bounds__(NW * 64) void items_kernel(Args A) {
   }
 }
 
-// Join of a row's items: one wave a row.  A row behind the last sequence, and a row that sees no key, is
+// Join of a row's items: one wave a row, bounded by the read of the parts (17 us for 256 rows of 64 heads: 9 parts of
+// 8.4 MB, 4.5 TB/s).  A row behind the last sequence, and a row that sees no key, is
 // zero (lse -inf).  A row of a sequence that brings more tokens than the call allows is NaN.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_kernel(Args A, int nw) {
@@ -985,8 +992,9 @@ PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, i
   out[0] = (int)ntp;
   if (wide) {
     // Beside own keys one round of blocks on 3/4 of the CUs, while the rest stream the own pages (256 sequences
-    // behind 32768 shared keys and 500 .. 1500 of their own: 531 us; 573 with 256 blocks, 599 with 512); alone, two
-    // rounds.  At least 1024 keys a block: 8192 keys in ranges of 512 take 76 us beside 64 sequences, of 1024 70.
+    // behind 32768 shared keys and 500 .. 1500 of their own: 447 us; 508 with 256 blocks, 524 with 512, 571 with
+    // 128); alone, two rounds.  At least 1024 keys a block: 8192 keys in ranges of 512 take 65 us beside 64
+    // sequences, of 1024 61.
     const long long cap = (plen + 1023) / 1024, n = (own > 0 ? 192 : 512) / (Hkv * ntp);
     out[1] = plen <= 0 ? 0 : (int)(n < 1 ? 1 : (n > cap ? cap : n));
   } else {

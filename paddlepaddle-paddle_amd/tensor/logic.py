@@ -148,7 +148,8 @@ def filtered_sampling(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     ones with at least ``min_p`` of the largest probability (0: all).  The answer is the first token, in the order of
     the vocabulary, at which the kept mass passes uniform times its total.  A temperature of 0 takes the largest logit
     (the lowest index of equal ones).  Tokens of -inf and NaN are never taken; a row that has no other gives token -1
-    and probability 0.  Sums are 64-bit: the answer does not depend on the device or on the order of addition.
+    and probability 0.  Sums are 64-bit: the answer does not depend on the order of addition.  (The
+    kernel takes no token under 2^-47 of the largest probability.)
 
     Returns (probs float32, ids int64), both [rows, 1]: the tokens and their shares of the kept mass.  Inference
     only: no gradient flows.  Beside ``top_p_sampling`` (probabilities in, its own random numbers)."""

@@ -409,6 +409,26 @@ def test_attention_refusals(dev):
     assert none._t.shape == (0, 4, 64)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('cu', [[0, 5, 3, 8], [-3, 2, 4, 8], [0, 9, 9, 12], [2 ** 31 - 1, -2 ** 31, 5, 8], [0, 0, 0, 0]])
+def test_offsets_that_do_not_fit(cu):
+    """Offsets that fall, start before the first row or end behind the last: nothing outside the tensors is read or
+    written (the queries of a sequence with such offsets are not defined), the caches' other places stay."""
+    g = torch.Generator().manual_seed(9)
+    kc, vc, tables, common = paged(g, [40, 40, 40], 16, 2, 64, BF, spare=3)
+    qkv = torch.randn(8, 8 * 64, generator=g).to(BF).cuda()
+    cu, lens, old = torch.tensor(cu, dtype=torch.int32).cuda(), torch.tensor([4, 5, 6], dtype=torch.int32).cuda(), kc.clone()
+    dk, dv, tables = kc.cuda(), vc.cuda(), tables.cuda()
+    q, _, _ = IF.paged_rotary_append(qkv, dk, dv, tables, lens, cu, frequencies(8).cuda())
+    common = common.cuda()
+    assert q._t.shape == (8, 4, 64) and torch.equal(dk[common.long()].cpu(), old[common.cpu().long()])
+    out = IF.shared_prefix_attention(q, dk, dv, tables, lens, common, 40, cu, 8)
+    torch.cuda.synchronize()
+    assert out._t.shape == (8, 4, 64)
+    if int(cu.abs().sum()) == 0:
+        assert float(out._t.float().abs().sum()) == 0.0
+
+
 # ------------------------------------------------------------------------------------------ sampling
 def sampling_case(dev, x, u, t, k, p, m):
     probs, ids = paddle.filtered_sampling(x.to(dev), u.to(dev), *(v.to(dev) if isinstance(v, torch.Tensor) else v
