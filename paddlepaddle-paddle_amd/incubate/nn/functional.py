@@ -932,8 +932,9 @@ def _check(ok, name, what):
 
 
 def _same_device(name, first, **others):
+    at = first.get_device()
     for k, t in others.items():
-        if isinstance(t, torch.Tensor) and t.device != first.device:
+        if isinstance(t, torch.Tensor) and t.get_device() != at:
             raise ValueError(f"{name}: {k} is on {t.device}, the input on {first.device}")
 
 

@@ -223,10 +223,13 @@ def stream():
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
+_HERE = contextlib.nullcontext()
+
+
 def device_of(t):
     """Context in which launches go to the device that holds ``t`` (which may not be the current one)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if t.get_device() == torch.cuda.current_device():
+        return _HERE
     return torch.cuda.device(t.device)
 
 
@@ -235,7 +238,7 @@ def ptr(t):
     meta tensor recorded into a static Program) raises here instead of reaching a kernel."""
     if t is None:
         return None
-    if t.device.type != 'cuda':
+    if not t.is_cuda:
         raise RuntimeError(f"HIP kernel operand on {t.device} (expected a GPU tensor)")
     return t.data_ptr()
 

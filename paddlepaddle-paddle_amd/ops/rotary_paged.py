@@ -25,7 +25,11 @@ def _alignment(ts):
     a = 8
     for t in ts:
         if t is not None and t.numel():
-            a = math.gcd(a, t.data_ptr() // t.element_size(), *(s for s, n in zip(t.stride()[:-1], t.shape) if n > 1))
+            a = math.gcd(a, t.data_ptr() // t.element_size())
+            if t.is_contiguous():
+                a = math.gcd(a, t.shape[-1])
+            else:
+                a = math.gcd(a, *(s for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1))
     return a
 
 
