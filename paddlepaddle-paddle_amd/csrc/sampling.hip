@@ -354,7 +354,7 @@ constexpr int CAP = 1024; // tokens of a border's bin that are listed
 constexpr int MC = 64;    // chunks whose scales are held at a time
 constexpr int WITH = 1024;  // parts that are looked through at a time
 
-constexpr int SUB = 512;  // tokens of a part of a chunk: a wave's 8 a lane
+constexpr int SUB = 128;  // tokens of a part of a chunk: 16 lanes' 8 each
 struct Chunk {
   uint32_t key, valid, first, pad;  // largest key, tokens, lowest index of the largest
   uint32_t part[CH / SUB];          // largest key of each part
@@ -389,14 +389,13 @@ __device__ __forceinline__ Grid grid_of(uint32_t key, double t) {
   g.top = x < INFINITY ? floor(x * g.s8) : INFINITY;  // (also where s8 is 0)
   return g;
 }
-// 2^(f / 8) scaled by 2^48 and rounded, by its Taylor series around the middle (relative error under 10^-15): what a
+// 2^(f / 8) scaled by 2^48 and rounded, by its Taylor series around the middle (relative error under 10^-13): what a
 // token adds to its bin's mass
 constexpr double kPart = 281474976710656.0;
 __device__ __forceinline__ unsigned long long part_mass(double f) {
   const double h = (f - 0.5) * 0.0866433975699931636771;  // ln 2 / 8
   constexpr double c = 1.0442737824274138403 * kPart;     // 2^(1 / 16)
-  double p = c / 5040.0;
-  p = fma(p, h, c / 720.0);
+  double p = c / 720.0;
   p = fma(p, h, c / 120.0);
   p = fma(p, h, c / 24.0);
   p = fma(p, h, c / 6.0);
@@ -452,8 +451,10 @@ __device__ __forceinline__ bool vector_rows(const Args& A) {
 }
 
 // What bounds it: 64-bit arithmetic, some 20 operations a token (a 32-bit mass would move the borders).  64 rows of
-// 128256 tokens in bf16 19 us, 512 rows of 32000 in fp32 30 us (2.2 TB/s), one row of 50304 9 us.  With one atomic for
-// count and mass instead of two 18 and 29, with four copies of the bins the same: the atomics are not what it waits for.
+// 128256 tokens in bf16 18 us, 512 rows of 32000 in fp32 29 us (2.3 TB/s), one row of 50304 9 us.  With one atomic for
+// count and mass instead of two, and with four copies of the bins, a twentieth less: the atomics are not what it waits
+// for.  Lists of a chunk's largest 128 tokens, written here, save the row's block 16 of 50 us at 128256 tokens and cost
+// 6 here, and at 32000 they cost 8 and save none: the row's block looks the tokens up by the maxima of parts instead.
 template <typename T>
 __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ out, int nc) {
   const int r = blockIdx.x / nc, ch = blockIdx.x % nc, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -472,13 +473,14 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
     ri = 0xffffffffu;
   }
   constexpr int E = 8, P = CH / (256 * E);  // a thread's tokens: P times E in a row, a wave's: P parts
-  static_assert(SUB == 64 * E, "a part is a wave's");
+  static_assert(SUB == 16 * E && CH / SUB == 64, "a part is 16 lanes', a chunk's parts a wave's lanes");
   T v[P][E];
   const bool vec = vector_rows<T>(A);
   uint32_t valid = 0;
 #pragma unroll
   for (int j = 0; j < P; ++j) load_tokens<T, E>(x, i0 + (j * 256 + tid) * E, end, vec, v[j]);
   __syncthreads();
+  uint32_t most[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     uint32_t m = 0;
@@ -488,20 +490,24 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
       valid += k != 0;
       m = max(m, k);
     }
-    m = wave_max_u(m);
-    if (lane == 0) {
-      rk[j * 4 + wave] = m;
-      C->part[j * 4 + wave] = m;
+    most[j] = m;
+    m = max(m, from_lane<0x111, 0xf>(m));  // over the 16 lanes, in the last of them
+    m = max(m, from_lane<0x112, 0xf>(m));
+    m = max(m, from_lane<0x114, 0xf>(m));
+    m = max(m, from_lane<0x118, 0xf>(m));
+    if ((lane & 15) == 15) {
+      rk[j * 16 + (tid >> 4)] = m;
+      C->part[j * 16 + (tid >> 4)] = m;
     }
   }
   valid = wave_add(valid);
   if (lane == 0) atomicAdd(&rv, valid);
   __syncthreads();
   valid = rv;
-  const uint32_t mk = wave_max_u(lane < CH / SUB ? rk[lane] : 0u);
+  const uint32_t mk = wave_max_u(rk[lane]);
 #pragma unroll
   for (int j = 0; j < P; ++j)
-    if (rk[j * 4 + wave] == mk && mk != 0) {  // the part has it
+    if (most[j] == mk && mk != 0) {  // the thread has it
 #pragma unroll
       for (int e = E - 1; e >= 0; --e)
         if (key_of(to_f(v[j][e])) == mk) atomicMin(&ri, (uint32_t)(i0 + (j * 256 + tid) * E + e));
@@ -538,9 +544,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
 }
 
 // Bounded by latency: some ten dependent steps over a few KB, one re-read of the parts that have a border's tokens, and
-// one chunk's scan.  One row of 50304 tokens 20 us (4 the first loads, 3 the join of the histograms, 5 the list, 1 each
-// selection); 64 rows of 128256 47 us, of which the list up to 19 (200 parts of 512 tokens by 8 waves, 4 in flight
-// each); 512 rows of 32000 44 us.
+// one chunk's scan.  One row of 50304 tokens 19 us (4 the first loads, 3 the join of the histograms, 5 the list, 1 each
+// selection); 64 rows of 128256 38 .. 47 us, as their longest list is; 512 rows of 32000 45 us.
 template <typename T>
 __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restrict__ in, int nc) {
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -681,22 +686,26 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     for (int p0 = 0; p0 < nc * PP; p0 += WITH) {
       if (tid == 0) wn = 0;
       __syncthreads();
-      for (int p = p0 + tid; p < min(p0 + WITH, nc * PP); p += NT) {
-        const uint32_t k = C[p / PP].part[p % PP];
-        if (k != 0 && value_of(k) >= from) with[atomicAdd(&wn, 1)] = p;
+      for (int p = p0 + tid; p - tid < min(p0 + WITH, nc * PP); p += NT) {
+        const uint32_t k = p < nc * PP ? C[p / PP].part[p % PP] : 0;
+        const unsigned long long in = __ballot(k != 0 && value_of(k) >= from);
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&wn, __popcll(in));
+        at = lane_value(at, 0) + __popcll(in & ((1ull << lane) - 1));
+        if (in >> lane & 1) with[at] = p;
       }
       __syncthreads();
       const int n = wn;
-      // PF parts of a wave are on their way at once: as many bytes as its registers take
+      // PF times 4 parts of a wave are on their way at once: as many bytes as its registers take
       constexpr int PF = sizeof(T) == 2 ? 4 : 2;
 #pragma unroll 1
-      for (int g = wave; g < n; g += PF * NW) {
+      for (int g = 4 * wave; g < n; g += 4 * PF * NW) {
         T raw[PF][8];
         int first[PF];
 #pragma unroll
         for (int k = 0; k < PF; ++k) {
-          const int j = g + k * NW;
-          first[k] = j < n ? with[j] * SUB + lane * 8 : A.V;
+          const int j = g + 4 * k * NW + (lane >> 4);
+          first[k] = j < n ? with[j] * SUB + (lane & 15) * 8 : A.V;
           load_tokens<T, 8>(x, first[k], A.V, vec, raw[k]);
         }
         auto in = [&](int k, int e) {
@@ -724,7 +733,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
       }
       __syncthreads();
     }
-    if (ln > CAP) return false;
+    if (ln != cum[b1] - (b0 ? cum[b0 - 1] : 0u)) return false;  // (not seen; what follows relies on it)
     uint32_t hi = 0, lo = 0xffffffffu;
     for (uint32_t i = tid; i < ln; i += NT) {
       const uint32_t id = (uint32_t)list[i].place, k = key_of(to_f(x[id]));
