@@ -375,12 +375,6 @@ struct Grid {
     double f;
     return bin(x, f);
   }
-  // weight, with 1 at the top of bin 0
-  __device__ __forceinline__ double weight(float x) const {
-    double f;
-    const int b = bin(x, f);
-    return exp2_64((f - 1.0 - (double)b) * 0.125);
-  }
 };
 __device__ __forceinline__ Grid grid_of(uint32_t key, double t) {
   Grid g;
@@ -389,10 +383,9 @@ __device__ __forceinline__ Grid grid_of(uint32_t key, double t) {
   g.top = x < INFINITY ? floor(x * g.s8) : INFINITY;  // (also where s8 is 0)
   return g;
 }
-// 2^(f / 8) scaled by 2^48 and rounded, by its Taylor series around the middle (relative error under 10^-13): what a
-// token adds to its bin's mass
+// 2^(f / 8) scaled by 2^48, by its Taylor series around the middle (relative error under 10^-13), plus `more`
 constexpr double kPart = 281474976710656.0;
-__device__ __forceinline__ unsigned long long part_mass(double f) {
+__device__ __forceinline__ double part(double f, double more) {
   const double h = (f - 0.5) * 0.0866433975699931636771;  // ln 2 / 8
   constexpr double c = 1.0442737824274138403 * kPart;     // 2^(1 / 16)
   double p = c / 720.0;
@@ -401,8 +394,17 @@ __device__ __forceinline__ unsigned long long part_mass(double f) {
   p = fma(p, h, c / 6.0);
   p = fma(p, h, c / 2.0);
   p = fma(p, h, c);
-  p = fma(p, h, c + 4503599627370496.0);  // on 2^52, whose last place is 1
-  return __builtin_bit_cast(unsigned long long, p) & 0xfffffffffffffull;
+  return fma(p, h, c + more);
+}
+// rounded: what a token adds to its bin's mass
+__device__ __forceinline__ unsigned long long part_mass(double f) {
+  return __builtin_bit_cast(unsigned long long, part(f, 4503599627370496.0)) & 0xfffffffffffffull;  // (on 2^52, whose last place is 1)
+}
+// a token's weight, with 1 at the upper end of bin 0; scale: of the bins' masses
+__device__ __forceinline__ double weight(const Grid& G, const double* scale, float x) {
+  double f;
+  const int b = G.bin(x, f);
+  return part(f, 0.0) * scale[b];
 }
 // w scaled by 2^49 and rounded, for w in [0, 1]: a listed token's mass
 constexpr double kFix = 562949953421312.0;
@@ -544,8 +546,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
 }
 
 // Bounded by latency: some ten dependent steps over a few KB, one re-read of the parts that have a border's tokens, and
-// one chunk's scan.  One row of 50304 tokens 19 us (4 the first loads, 3 the join of the histograms, 5 the list, 1 each
-// selection); 64 rows of 128256 38 .. 47 us, as their longest list is; 512 rows of 32000 45 us.
+// one chunk's scan.  One row of 50304 tokens 18 us (4 the first loads, 3 the join of the histograms, 5 the list, 1 each
+// selection); 64 rows of 128256 38 .. 45 us, as their longest list is; 512 rows of 32000 43 us.
 template <typename T>
 __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restrict__ in, int nc) {
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -611,7 +613,6 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     return;
   }
   const Grid G = grid_of(mk, S.t);
-  const double wmax = G.weight(value_of(mk));
   // the shifts of the bins of chunks [c0, c0 + MC)
   auto shifts = [&](int c0) {
     __syncthreads();
@@ -737,7 +738,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     uint32_t hi = 0, lo = 0xffffffffu;
     for (uint32_t i = tid; i < ln; i += NT) {
       const uint32_t id = (uint32_t)list[i].place, k = key_of(to_f(x[id]));
-      list[i] = Token{place(k, id), fixed(G.weight(value_of(k)))};
+      list[i] = Token{place(k, id), fixed(weight(G, scale, value_of(k)))};
       hi = max(hi, k);
       lo = min(lo, k);
     }
@@ -881,7 +882,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     const double d = G.top - floor((double)value_of(mk) * G.s8 + 8.0 * log2(S.m));
     bm = d < (double)(NB - 1) ? max((int)d, 0) : (d != d ? 0 : NB - 1);
   }
-  const double least = S.m * wmax;  // by min-p
+  const double least = S.m * weight(G, scale, value_of(mk));  // by min-p
   // Drops what min-p or a place cuts off the list; returns the mass that is left
   auto keep = [&](unsigned long long tp) -> unsigned long long {
     __syncthreads();
@@ -889,7 +890,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     __syncthreads();
     unsigned long long w = 0;
     for (uint32_t i = tid; i < ln; i += NT) {
-      if (list[i].place < tp || !(G.weight(value_of((uint32_t)(list[i].place >> 32))) >= least)) list[i].w = 0;
+      if (list[i].place < tp || !(weight(G, scale, value_of((uint32_t)(list[i].place >> 32))) >= least)) list[i].w = 0;
       w += list[i].w;
     }
     w = wave_add(w);
@@ -945,7 +946,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     if (step == 2) {
       if (tid == 0) {
         A.ids[r] = (int64_t)(0xffffffffu - (uint32_t)q);
-        A.probs[r] = (float)(G.weight(value_of((uint32_t)(q >> 32))) / ((double)sum * (1.0 / kFix)));
+        A.probs[r] = (float)(weight(G, scale, value_of((uint32_t)(q >> 32))) / ((double)sum * (1.0 / kFix)));
       }
       return;
     }
@@ -1016,7 +1017,7 @@ __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restr
     const uint32_t k = key_of(q);
     const int b = k != 0 ? G.bin(q) : NB;
     if (!(b < bf || (partial && b == bf))) return 0.0;
-    const double w = G.weight(q);
+    const double w = weight(G, scale, q);
     return b < bf || passes(place(k, i), w) ? w : 0.0;
   };
   double each[E], sum = 0.0;
