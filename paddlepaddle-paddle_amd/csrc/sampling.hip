@@ -151,7 +151,8 @@ __device__ __forceinline__ Setting setting(const Args& A, int r) {
   const int k = A.k[r];
   Setting c;
   c.t = temperature(A, r);
-  c.p = A.own & 4 ? (double)p : A.p0;
+  const double p_ = A.own & 4 ? (double)p : A.p0;
+  c.p = p_ > 0.0 ? p_ : 0.0;  // (NaN: the first token alone)
   const double m = A.own & 8 ? (double)m_ : A.m0;
   const uint64_t w = (uint64_t)__builtin_bit_cast(uint32_t, u32b) << 32 | __builtin_bit_cast(uint32_t, u32);
   const double u = A.u64 ? __builtin_bit_cast(double, w) : (double)u32;

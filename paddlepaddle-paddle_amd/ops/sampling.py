@@ -46,7 +46,7 @@ def composite(x, u, temperature, top_k, top_p, min_p):
 
 
 def sample(x, u, temperature, top_k, top_p, min_p):
-    """x [rows, V]; u [rows]; the settings scalars or [rows] tensors.  Returns (probs fp32, ids int64), [rows, 1]."""
+    """x [rows, V]; u [rows]; the settings scalars or [rows] tensors (fp32, top_k int32).  Returns (probs fp32, ids int64), [rows, 1]."""
     rows, V = x.shape
     if not _hip(x):
         with torch.no_grad():
@@ -55,13 +55,12 @@ def sample(x, u, temperature, top_k, top_p, min_p):
     u = (u if u.dtype in (torch.float32, torch.float64) else u.float()).contiguous()
     keep = []
 
-    def setting(v, dt):
+    def setting(v):
         if not isinstance(v, torch.Tensor):
             return None, v
-        keep.append(v.to(dt).contiguous())
+        keep.append(v.contiguous())
         return N.ptr(keep[-1]), 0
-    (tp, t0), (kp, k0), (pp, p0), (mp, m0) = (setting(temperature, torch.float32), setting(top_k, torch.int32),
-                                              setting(top_p, torch.float32), setting(min_p, torch.float32))
+    (tp, t0), (kp, k0), (pp, p0), (mp, m0) = (setting(v) for v in (temperature, top_k, top_p, min_p))
     ids = torch.empty(rows, 1, dtype=torch.int64, device=x.device)
     probs = torch.empty(rows, 1, dtype=torch.float32, device=x.device)
     if rows == 0:

@@ -141,7 +141,8 @@ def top_p_sampling(x, ps, threshold=None, topp_seed=None, seed=-1, k=0, mode='tr
 
 def filtered_sampling(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, name=None):
     """One token per row of logits x [rows, vocab], from given random numbers ``uniform`` [rows] (or [rows, 1]) in
-    [0, 1), after temperature, top-k, top-p and min-p; every setting is a number or a tensor of one per row.
+    [0, 1), after temperature, top-k, top-p and min-p; every setting is a number or a tensor of one per row (taken in 32
+    bits).
 
     Of the tokens in the order of falling logits (equal ones: the lower index first) the first ``top_k`` are kept (0:
     all), of those the ones before which less than ``top_p`` of their mass lies (1: all; at least one), of those the
@@ -164,13 +165,15 @@ def filtered_sampling(x, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     def setting(v, what, whole=False):
         v = _u(v)
         if not isinstance(v, torch.Tensor):
-            return int(v) if whole else float(v)
+            return max(0, min(int(v), 2 ** 31 - 1)) if whole else float(v)
         if v.numel() != t.shape[0] or v.is_floating_point() == whole:
             raise ValueError(f"filtered_sampling: {what} must be a number or {t.shape[0]} "
                              f"{'integers' if whole else 'floating numbers'}, got {v.dtype} {list(v.shape)}")
         if v.device != t.device:
             raise ValueError(f"filtered_sampling: {what} is on {v.device}, x on {t.device}")
-        return v.reshape(-1)
+        if whole:
+            return (v if v.dtype == torch.int32 else v.clamp(0, 2 ** 31 - 1).to(torch.int32)).reshape(-1)
+        return v.reshape(-1).float()
     if u.device != t.device:
         raise ValueError(f"filtered_sampling: uniform is on {u.device}, x on {t.device}")
     settings = (setting(temperature, 'temperature'), setting(top_k, 'top_k', True), setting(top_p, 'top_p'),

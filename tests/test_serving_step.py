@@ -523,6 +523,35 @@ def test_sampling_strided_rows_and_empty(dev):
 
 
 @pytest.mark.parametrize('dev', DEVICES)
+def test_sampling_settings_of_other_types(dev):
+    g = torch.Generator().manual_seed(10)
+    x, u = torch.randn(4, 300, generator=g), torch.rand(4, generator=g)
+    nan = float('nan')
+
+    def run(*settings):
+        probs, ids = paddle.filtered_sampling(x.to(dev), u.to(dev), *(v.to(dev) if isinstance(v, torch.Tensor) else v
+                                                                      for v in settings))
+        return ids._t.cpu().reshape(-1).tolist(), probs._t.cpu()
+    full = lambda v, t: torch.full((4,), v, dtype=t)  # noqa: E731
+    plain = run(0.8, 0, 0.9, 0.01)
+    for k in (2 ** 40 + 3, -2 ** 40 + 3, full(2 ** 40 + 3, torch.int64), full(-2 ** 40 + 3, torch.int64)):  # all
+        assert run(0.8, k, 0.9, 0.01)[0] == plain[0]
+    for t in (torch.float64, torch.float32):
+        same = run(full(0.75, t), full(7, torch.int64), full(0.5, t), full(0.125, t))
+        want = run(0.75, 7, 0.5, 0.125)
+        assert same[0] == want[0] and torch.equal(same[1], want[1])
+    first = x.argmax(-1).tolist()
+    assert run(nan, 0, 1.0, 0.0)[0] == first and run(1.0, 0, nan, 0.0)[0] == first and run(1.0, 0, full(nan, FF), 0.0)[0] == first
+    assert run(0.8, 0, 0.9, nan)[0] == run(0.8, 0, 0.9, 0.0)[0]
+    paddle_u = paddle.filtered_sampling(x.to(dev), full(nan, FF).to(dev))[1]._t.cpu().reshape(-1).tolist()
+    assert paddle_u == [0] * 4
+    # columns and expanded numbers as settings
+    wide = torch.rand(4, 3, generator=g) + 0.5
+    want = [O.sample(x[r], float(u[r]), float(wide[r, 1]), 9, 0.875, 0.0)[0] for r in range(4)]
+    assert run(wide[:, 1], torch.tensor(9, dtype=torch.int32).expand(4), torch.tensor([0.875]).expand(4), 0.0)[0] == want
+
+
+@pytest.mark.parametrize('dev', DEVICES)
 def test_sampling_refusals(dev):
     x, u = torch.randn(3, 9, device=dev), torch.rand(3, device=dev)
     for bad in ((x[0], u), (x.double(), u), (x[:, :0], u), (x, u[:2]), (x, u.long()), (x, 0.5)):
