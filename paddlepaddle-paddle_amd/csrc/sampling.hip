@@ -370,7 +370,9 @@ struct Grid {
     const double g = floor((double)x * s8), d = top - g;
     // (written out: the same weight wherever it is computed; NaN, of infinities: 0; places from 2^53 on: any of [0, 1])
     f = fmin(fmax(fma((double)x, s8, -g), 0.0), 1.0);
-    return d < (double)(NB - 1) ? (int)d : (d != d ? 0 : NB - 1);
+    int b;
+    asm("v_cvt_i32_f64 %0, %1" : "=v"(b) : "v"(d));  // NaN: 0; beyond the integers: the largest
+    return min(b, NB - 1);
   }
   __device__ __forceinline__ int bin(float x) const {
     double f;
@@ -384,18 +386,32 @@ __device__ __forceinline__ Grid grid_of(uint32_t key, double t) {
   g.top = x < INFINITY ? floor(x * g.s8) : INFINITY;  // (also where s8 is 0)
   return g;
 }
-// 2^(f / 8) scaled by 2^48, by its Taylor series around the middle (relative error under 10^-13), plus `more`
+// 2^(f / 8) scaled by 2^48, plus `more`: its Taylor polynomial around the middle (relative error under 10^-13), multiplied
+// out to powers of f
 constexpr double kPart = 281474976710656.0;
+struct Powers {
+  double c[7];
+  constexpr Powers() : c{} {
+    const double a = 0.0866433975699931636771;      // ln 2 / 8
+    double t = 1.0442737824274138403 * kPart;       // 2^(1 / 16) a^k / k!
+    for (int k = 0; k < 7; ++k, t *= a / k) {
+      double w = t;                                 // of (f - 1/2)^k: binomial(k, j) (-1/2)^(k - j) f^j
+      for (int j = k; j >= 0; --j) {
+        c[j] += w;
+        w *= -0.5 * j / (k - j + 1);
+      }
+    }
+  }
+};
 __device__ __forceinline__ double part(double f, double more) {
-  const double h = (f - 0.5) * 0.0866433975699931636771;  // ln 2 / 8
-  constexpr double c = 1.0442737824274138403 * kPart;     // 2^(1 / 16)
-  double p = c / 720.0;
-  p = fma(p, h, c / 120.0);
-  p = fma(p, h, c / 24.0);
-  p = fma(p, h, c / 6.0);
-  p = fma(p, h, c / 2.0);
-  p = fma(p, h, c);
-  return fma(p, h, c + more);
+  constexpr Powers P;
+  double p = P.c[6];
+  p = fma(p, f, P.c[5]);
+  p = fma(p, f, P.c[4]);
+  p = fma(p, f, P.c[3]);
+  p = fma(p, f, P.c[2]);
+  p = fma(p, f, P.c[1]);
+  return fma(p, f, P.c[0] + more);
 }
 // rounded: what a token adds to its bin's mass
 __device__ __forceinline__ unsigned long long part_mass(double f) {
@@ -453,8 +469,8 @@ __device__ __forceinline__ bool vector_rows(const Args& A) {
   return (reinterpret_cast<uintptr_t>(A.x) & 15) == 0 && A.row % (16 / (int)sizeof(T)) == 0;
 }
 
-// What bounds it: 64-bit arithmetic, some 20 operations a token (a 32-bit mass would move the borders).  64 rows of
-// 128256 tokens in bf16 18 us, 512 rows of 32000 in fp32 29 us (2.3 TB/s), one row of 50304 9 us.  With one atomic for
+// What bounds it: 64-bit arithmetic, some 13 operations a token (a 32-bit mass would move the borders).  64 rows of
+// 128256 tokens in bf16 17 us, 512 rows of 32000 in fp32 27 us (2.4 TB/s), one row of 50304 8 us.  With one atomic for
 // count and mass instead of two, and with four copies of the bins, a twentieth less: the atomics are not what it waits
 // for.  Lists of a chunk's largest 128 tokens, written here, save the row's block 16 of 50 us at 128256 tokens and cost
 // 6 here, and at 32000 they cost 8 and save none: the row's block looks the tokens up by the maxima of parts instead.
@@ -548,7 +564,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
 
 // Bounded by latency: some ten dependent steps over a few KB, one re-read of the parts that have a border's tokens, and
 // one chunk's scan.  One row of 50304 tokens 18 us (4 the first loads, 3 the join of the histograms, 5 the list, 1 each
-// selection); 64 rows of 128256 38 .. 45 us, as their longest list is; 512 rows of 32000 43 us.
+// selection); 64 rows of 128256 38 .. 45 us, as their longest list is; 512 rows of 32000 41 us.
 template <typename T>
 __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restrict__ in, int nc) {
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
