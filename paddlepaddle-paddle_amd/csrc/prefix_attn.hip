@@ -108,10 +108,11 @@ __device__ __forceinline__ void dma_tile(const char* base, const unsigned (&off)
         "global_load_lds_dwordx4 %1, %5\n\t"
         "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
         "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-        "global_load_lds_dwordx4 %4, %5 offset:3072\n\t"
+        "global_load_lds_dwordx4 %4, %5 offset:%7\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(keep)
-        : "v"(off[i]), "v"(off[i + 1]), "v"(off[i + 2]), "v"(off[i + 3]), "s"(base), "s"(dst + i * 1024)
+        : "v"(off[i]), "v"(off[i + 1]), "v"(off[i + 2]), "v"(off[i + 3]), "s"(base), "s"(dst + i * 1024),
+          "n"(3 * 1024)
         : "memory");
   }
 }
