@@ -34,13 +34,14 @@ __device__ __forceinline__ float2 angle(const double* inv_freq, float scale, lon
 // Units of a head: `nr` that turn (V values and their V partners at + pairs in the half layout, V values of
 // interleaved pairs), then the copied ones of V values.  A thread's units of the block's token, in order:
 struct Walk {
-  int units, nr, heads, Ht;  // heads: taken at once
+  int threads, units, nr, heads, Ht;  // heads: taken at once
   int u, hh, hl;             // the next unit, its head
   bool more;
-  __device__ __forceinline__ Walk(int V, bool inter, int D, int pairs, int Ht_) {
+  __device__ __forceinline__ Walk(int V, bool inter, int D, int pairs, int Ht_, int threads_) {
+    threads = threads_;
     nr = (inter ? 2 * pairs : pairs) / V;
     units = nr + (D - 2 * pairs) / V;
-    heads = units < 256 ? 256 / units : 1;
+    heads = units < threads ? threads / units : 1;
     Ht = Ht_;
     hl = threadIdx.x / units;
     u = threadIdx.x % units;
@@ -51,7 +52,7 @@ struct Walk {
     hh += heads;
     if (hh < Ht) return;
     hh = hl;
-    u += 256;  // only where a head has over 256 units
+    u += threads;  // only where a head has more units than the block threads
     more = u < units;
   }
   template <int V, bool INTER>
@@ -146,7 +147,7 @@ struct RopeArgs {
   const void* pos;  // int32 / int64 [B, S] of the given strides, or null: the token's index
   long long ps[2];
   int pos64;
-  int S, D, pairs;
+  int S, D, pairs, threads;
   long long tokens;
   float sign, scale;
   const double* inv_freq;
@@ -162,14 +163,14 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs A) {
   T* const y0 = reinterpret_cast<T*>(A.y[0]) + tok * A.H[0] * A.D;
   T* const y1 = reinterpret_cast<T*>(A.y[1]) + tok * A.H[1] * A.D;
   stream<T, V, INTER, 4>(
-      Walk(V, INTER, A.D, A.pairs, A.H[0] + A.H[1]), A.pairs,
+      Walk(V, INTER, A.D, A.pairs, A.H[0] + A.H[1], A.threads), A.pairs,
       [&](int hh) { return hh < A.H[0] ? x0 + hh * A.xs[0][2] : x1 + (hh - A.H[0]) * A.xs[1][2]; },
       [&]() {
         long long p = s;
         if (A.pos)
           p = A.pos64 ? reinterpret_cast<const int64_t*>(A.pos)[b * A.ps[0] + s * A.ps[1]]
                       : (long long)reinterpret_cast<const int32_t*>(A.pos)[b * A.ps[0] + s * A.ps[1]];
-        for (int i = threadIdx.x; i < A.pairs; i += 256) cs[i] = angle(A.inv_freq, A.scale, p, i, A.sign);
+        for (int i = threadIdx.x; i < A.pairs; i += A.threads) cs[i] = angle(A.inv_freq, A.scale, p, i, A.sign);
         __syncthreads();
       },
       [&](int hh, int off, bool turn, const Pack<T, V>& a, const Pack<T, V>& b) {
@@ -193,7 +194,7 @@ struct AppendArgs {
   const int* cu;    // [B + 1] or null: one token each
   const int* off_dev;
   long long off;  // position = off + place in the cache
-  int T, B, Hq, Hkv, D, pairs;
+  int T, B, Hq, Hkv, D, pairs, threads;
   float scale;
   const double* inv_freq;
 };
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs A) {
   bool in = false;     // the token belongs to a sequence
   long long dst = -1;  // where its keys go (element offset of head 0), -1: nowhere
   stream<T, V, INTER, 4>(
-      Walk(V, INTER, A.D, A.pairs, A.Hq + 2 * A.Hkv), A.pairs, [&](int hh) { return x + (long long)hh * A.D; },
+      Walk(V, INTER, A.D, A.pairs, A.Hq + 2 * A.Hkv, A.threads), A.pairs, [&](int hh) { return x + (long long)hh * A.D; },
       [&]() {
         // (each wave for itself: no barrier before the angles)
         const int b = A.cu ? __builtin_amdgcn_readfirstlane(seq_of_token(A.cu, A.B, t)) : (t < A.B ? t : A.B);
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs A) {
             if (blk >= 0 && blk < A.num_blocks) dst = blk * A.cs[0] + (p - pg * A.page) * A.cs[2];
           }
           p += A.off_dev ? (long long)*A.off_dev : A.off;
-          for (int i = threadIdx.x; i < A.pairs; i += 256) cs[i] = angle(A.inv_freq, A.scale, p, i, 1.f);
+          for (int i = threadIdx.x; i < A.pairs; i += A.threads) cs[i] = angle(A.inv_freq, A.scale, p, i, 1.f);
         }
         __syncthreads();
       },
@@ -272,6 +273,14 @@ using namespace pa::rot;
     else KERNEL<T, 1, false> __VA_ARGS__;                                                        \
   }
 
+// Threads of a token's block: as many waves as its units fill, up to 4 (65536 tokens of 4 + 4 heads of 64: 31 us with
+// one wave, 68 with four; 32768 of 8 + 2 heads of 128: 30 with two, 43 with four).  An argument of the kernel: the block's
+// size as the hardware tells it is a load more before the first data (80 heads of 128: 64 beside 61 us).
+inline int block_threads(int D, int pairs, bool inter, int heads, int v) {
+  const long long units = (long long)heads * ((inter ? 2 * pairs : pairs) / v + (D - 2 * pairs) / v);
+  return units <= 64 ? 64 : (units <= 128 ? 128 : 256);
+}
+
 // q / k: [B, S, H, D] views with unit inner stride and the given (batch, token, head) strides; yq / yk
 // contiguous.  `align`: elements that divide every stride and address.  sign -1: the backward pass.
 PA_API int pa_rope_freq(const void* q, const void* k, void* yq, void* yk, const long long* qs, const long long* ks,
@@ -291,7 +300,8 @@ PA_API int pa_rope_freq(const void* q, const void* k, void* yq, void* yk, const 
   const int v = width(dt == 0 ? 4 : 2, D, pairs, inter != 0, align);
   if (inter && (D % v || align % v)) return (int)hipErrorInvalidValue;  // pairs are loaded together
   if (A.tokens > 0x7fffffff) return (int)hipErrorInvalidValue;
-  PA_DISPATCH_DTYPE(dt, T, PA_ROT_LAUNCH(T, rope_kernel, <<<(int)A.tokens, 256, 0, st>>>(A)))
+  A.threads = block_threads(D, pairs, inter != 0, A.H[0] + A.H[1], v);
+  PA_DISPATCH_DTYPE(dt, T, PA_ROT_LAUNCH(T, rope_kernel, <<<(int)A.tokens, A.threads, 0, st>>>(A)))
   return (int)hipGetLastError();
 }
 
@@ -315,6 +325,7 @@ PA_API int pa_paged_append(const void* qkv, long long row, const void* bias, voi
   A.inv_freq = inv_freq; A.scale = scale;
   const int v = width(dt == 0 ? 4 : 2, D, pairs, inter != 0, align);
   if (inter && (D % v || align % v)) return (int)hipErrorInvalidValue;
-  PA_DISPATCH_DTYPE(dt, T_, PA_ROT_LAUNCH(T_, append_kernel, <<<T, 256, 0, st>>>(A)))
+  A.threads = block_threads(D, pairs, inter != 0, Hq + 2 * Hkv, v);
+  PA_DISPATCH_DTYPE(dt, T_, PA_ROT_LAUNCH(T_, append_kernel, <<<T, A.threads, 0, st>>>(A)))
   return (int)hipGetLastError();
 }
