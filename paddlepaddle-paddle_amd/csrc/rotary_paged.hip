@@ -273,12 +273,13 @@ using namespace pa::rot;
     else KERNEL<T, 1, false> __VA_ARGS__;                                                        \
   }
 
-// Threads of a token's block: as many waves as its units fill, up to 4 (65536 tokens of 4 + 4 heads of 64: 31 us with
-// one wave, 68 with four; 32768 of 8 + 2 heads of 128: 30 with two, 43 with four).  An argument of the kernel: the block's
-// size as the hardware tells it is a load more before the first data (80 heads of 128: 64 beside 61 us).
+// Threads of a token's block: two units a thread, up to 4 waves (65536 tokens of 4 + 4 heads of 64, 32 units: 31 us with
+// one wave, 44 with two, 69 with four; 32768 of 8 + 2 heads of 128, 80 units: 27, 30, 43; from 320 units on four waves
+// are as fast as one, and for few tokens faster: 16 of 48 heads of 128, 384 units: 6.2, 4.8, 4.2).  An argument of the
+// kernel: the block's size as the hardware tells it is a load more before the first data (80 heads of 128: 64 beside 61 us).
 inline int block_threads(int D, int pairs, bool inter, int heads, int v) {
   const long long units = (long long)heads * ((inter ? 2 * pairs : pairs) / v + (D - 2 * pairs) / v);
-  return units <= 64 ? 64 : (units <= 128 ? 128 : 256);
+  return units <= 128 ? 64 : (units <= 256 ? 128 : 256);
 }
 
 // q / k: [B, S, H, D] views with unit inner stride and the given (batch, token, head) strides; yq / yk
