@@ -508,6 +508,18 @@ def test_sampling_large_vocabularies(dev, vocab, dtype):
         sampling_case(dev, x, u, t, k, p, m)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('vocab,settings', [(150001, ((1.0, 0, 0.9, 0.0), (0.8, 700, 0.95, 0.0), (1.0, 0, 1.0, 0.0))),
+                                            (600007, ((1.0, 0, 0.5, 0.0), (0.7, 900, 1.0, 0.001), (2.0, 0, 1.0, 0.0)))])
+def test_sampling_vocabularies_of_many_chunks(vocab, settings):
+    """More parts than are looked through at a time (131072 tokens), more chunks than the shifts held (524288)."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(2, vocab, generator=g) * 2.5
+    x[1, vocab - 400:] += 4.0                        # the candidates lie in the last chunk
+    for t, k, p, m in settings:
+        sampling_case('cuda', x, torch.tensor([0.37, 0.992], dtype=torch.float64), t, k, p, m)
+
+
 @pytest.mark.parametrize('dev', DEVICES)
 def test_sampling_strided_rows_and_empty(dev):
     g = torch.Generator().manual_seed(9)
