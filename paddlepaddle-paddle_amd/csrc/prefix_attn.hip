@@ -20,6 +20,10 @@
 //
 // Keys past the range and keys of unallocated pages (table entries outside the cache) are read from a row
 // of zeros and masked: what lies in a page's unused slots never reaches a product.
+//
+// Offsets of a block, a head and a slot are 64-bit.  A tile's whole-page path adds its rows' offsets from the first row
+// in 32 bits, an instruction's rows in one page likewise; strides for which these do not fit (kTileStride, kRowStride)
+// take an address for each lane.
 #define PA_FA_PAIR_GROUP_DECL static __constant__
 #include "flash_attn_kernels.h"
 #include "paged.h"
@@ -30,6 +34,10 @@ namespace pfx {
 using fa::f32x4;
 using fa::s16x4;
 using fa::s16x8;
+
+// Largest slot strides (elements) for which the bytes from a tile's first row to the end of its last one, 63 rows on, are
+// under 2^32 (the narrow items' 31 rows: under 2^31), and to the end of a DMA instruction's last row, 7 on, under 2^31
+constexpr long long kTileStride = 1ll << 25, kRowStride = 1ll << 27;
 
 __device__ const uint16_t g_zero_row[256] __attribute__((aligned(16))) = {0};
 
@@ -256,12 +264,13 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
   // LDS-DMA of the 32 keys (or values) from kt on into the LDS image at dst: NI instructions on every path.
   // A lane fetches chunk cl ^ swizzle of its row; the swizzle is that of the image.  Returns the keys (bit r:
   // key kt + r) that exist.
-  const bool whole_page = A.page % 32 == 0 && A.cr >= D, grouped = A.page % SH::RPI == 0;
+  const bool whole_page = A.page % 32 == 0 && A.cr >= D && A.cr <= kTileStride,
+             grouped = A.page % SH::RPI == 0 && A.cr <= kRowStride;
   unsigned fk[SH::NI], fv[SH::NI];  // byte offsets of the fast path, less what the instruction's offset adds
 #pragma unroll
   for (int i = 0; i < SH::NI; ++i) {
     const int row = i * SH::RPI + rl;
-    const unsigned r = (unsigned)(row * (int)A.cr * 2 - (i & 3) * 1024);
+    const unsigned r = (unsigned)row * (unsigned)A.cr * 2 - (i & 3) * 1024;
     fk[i] = r + ((unsigned)(cl ^ fa::swz_b128<D>(row)) << 4);
     fv[i] = r + ((unsigned)(cl ^ fa::swz_tr<D>(row)) << 4);
   }
@@ -281,7 +290,7 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
                                      (unsigned long long)(unsigned)__builtin_amdgcn_readlane(hi, i * SH::RPI) << 32;
         const int row = i * SH::RPI + rl;
         const unsigned sw = (unsigned)(cl ^ (isv ? fa::swz_tr<D>(row) : fa::swz_b128<D>(row))) << 4;
-        fa::fa_glds(base + o, (unsigned)(rl * (int)A.cr * 2) + sw, dst + i * 1024);
+        fa::fa_glds(base + o, (unsigned)rl * (unsigned)A.cr * 2 + sw, dst + i * 1024);
       }
     } else {  // an address for each lane; rows that do not exist come from a row of zeros
       int ln = lane;
@@ -575,15 +584,15 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
   const char* const kh = reinterpret_cast<const char*>(A.kc + hk * A.ch);
   const char* const vh = reinterpret_cast<const char*>(A.vc + hk * A.ch);
   auto page_of = [&](int key) { return A.page_shift >= 0 ? key >> A.page_shift : key / A.page; };
-  const bool grouped = A.page % SH::RPI == 0;
+  const bool grouped = A.page % SH::RPI == 0 && A.cr <= kRowStride;
   Window win{A.ptable, A.pblocks, 0, -1};
   if (nt > 0) win.load(page_of(k0));
   unsigned sk[ND], sv[ND];  // byte offsets from the first row of an instruction
 #pragma unroll
   for (int i = 0; i < ND; ++i) {
     const int row = (wave * ND + i) * SH::RPI + rl;
-    sk[i] = (unsigned)(rl * (int)A.cr * 2) + ((unsigned)(cl ^ fa::swz_b128<D>(row)) << 4);
-    sv[i] = (unsigned)(rl * (int)A.cr * 2) + ((unsigned)(cl ^ fa::swz_tr<D>(row)) << 4);
+    sk[i] = (unsigned)rl * (unsigned)A.cr * 2 + ((unsigned)(cl ^ fa::swz_b128<D>(row)) << 4);
+    sv[i] = (unsigned)rl * (unsigned)A.cr * 2 + ((unsigned)(cl ^ fa::swz_tr<D>(row)) << 4);
   }
 
   // Places of a tile's 64 keys: byte offset of key kt + lane from the head's base, and which keys exist
@@ -591,7 +600,7 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
     unsigned lo, hi;
     unsigned long long ok;
   };
-  const bool aligned = A.page % 64 == 0;  // a tile lies in one page
+  const bool aligned = A.page % 64 == 0 && A.cr <= kTileStride;  // a tile lies in one page
   const unsigned lane_off = (unsigned)lane * (unsigned)A.cr * 2;
   auto places = [&](int kt) -> Places {
     if (aligned) {
@@ -1018,7 +1027,7 @@ PA_API int pa_prefix_attn(const void* q, const void* kc, const void* vc, long lo
                           const int* plan, int T, int B, int Hq, int Hkv, int D, int most, float scale, int dt,
                           hipStream_t st) {
   if (T <= 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || page <= 0 || num_blocks < 0 || (dt != 1 && dt != 2) ||
-      !(scale > 0.f) || cstr[2] > (1 << 27) || (!cu && T != B) || (plan[4] > 0 && !ws))
+      !(scale > 0.f) || cstr[2] < 0 || (!cu && T != B) || (plan[4] > 0 && !ws))
     return (int)hipErrorInvalidValue;
   Args A;
   A.q = (const uint16_t*)q; A.kc = (const uint16_t*)kc; A.vc = (const uint16_t*)vc;

@@ -1,0 +1,75 @@
+"""Operators of a serving step at the edges of what their documentation allows: other orders of a cache, far strides,
+wide integers, long tables, extreme scores."""
+import math
+
+import pytest
+import torch
+
+import paddle.incubate.nn.functional as IF
+
+import serving_oracle as O
+from test_serving_step import BF, DEVICES, FF, HF, frequencies, near, paged
+
+
+# ------------------------------------------------------------------------------------------ orders of a cache
+def slot_major(cache):
+    """The same cache in [block, slot, head, D] storage, seen as [block, head, slot, D]."""
+    return cache.transpose(1, 2).contiguous().transpose(1, 2)
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('hq,hkv,d,page,plen,own,new,dtype', [
+    (8, 4, 128, 64, 300, [70, 129, 1], None, BF),            # whole pages a tile, few rows
+    (12, 3, 64, 32, 130, [65, 40], [65, 3], HF),
+    (4, 2, 256, 64, 100, [64, 3], None, BF),
+    (32, 2, 128, 64, 333, [5, 70] * 8, None, BF),            # prefix items of many rows: pages of a tile, ...
+    (32, 2, 64, 16, 333, [5, 70] * 8, None, HF),             # ... of an instruction's rows, ...
+    (32, 2, 128, 5, 203, [5, 30] * 8, None, BF),             # ... and of neither
+    (16, 2, 256, 64, 200, [2, 33] * 8, None, BF),
+    (4, 2, 64, 5, 21, [13, 4], None, HF)])
+def test_slot_major_caches(dev, hq, hkv, d, page, plen, own, new, dtype):
+    """Appended to and read: slots Hkv * D apart, heads D apart."""
+    g = torch.Generator().manual_seed(hq * d + page)
+    n = [1] * len(own) if new is None else new
+    kc, vc, tables, common = paged(g, own, page, hkv, d, dtype, spare=-(-plen // page))
+    cu = None if new is None else torch.tensor([0] + n).cumsum(0).int()
+    lens, f = torch.tensor(own, dtype=torch.int32), frequencies(d // 4)
+    past = lens - torch.tensor(n, dtype=torch.int32)
+    qkv = torch.randn(sum(n), (hq + 2 * hkv) * d, generator=g).to(dtype)
+    wq, wk, wv = O.append(qkv, kc, vc, tables, past, cu, f, False, 1.0, plen)
+    dk, dv = slot_major(kc.to(dev)), slot_major(vc.to(dev))
+    assert dk.stride() == (page * hkv * d, d, hkv * d, 1)
+    up = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    q, k2, _ = IF.paged_rotary_append(up(qkv), dk, dv, up(tables), up(past), up(cu), up(f), position_offset=plen)
+    assert k2._t.data_ptr() == dk.data_ptr()
+    step = torch.finfo(dtype).eps / 2
+    near(q._t, wq, wq.abs() * step + 1e-5)
+    near(dk, wk, wk.abs() * step + 1e-5)
+    assert torch.equal(dv.cpu().double(), wv)
+    want, _, size = O.attention(q._t.cpu(), dk.cpu(), dv.cpu(), tables, lens, common, plen, cu, 1 / math.sqrt(d))
+    got = IF.shared_prefix_attention(q, dk, dv, up(tables), up(lens), up(common), plen, up(cu), max(n))
+    near(got._t, want, O.attention_bound(want, size, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows', [1, 20])                    # prefix items of few rows and of many
+@pytest.mark.parametrize('page,stride', [(64, 70_000_000), (16, (1 << 27) + 8), (64, (1 << 25) + 8), (64, 1 << 25)])
+def test_slot_strides_beyond_32_bits(page, stride, rows):
+    """Slots so far apart that a tile's rows lie up to 9 GB behind each other: a [slot, block, head, D] storage of many
+    blocks, of which a few are used."""
+    g = torch.Generator().manual_seed(page + rows)
+    hq, hkv, d, nblk = 8, 1, 128, 6
+    room = torch.empty(page * stride, dtype=BF, device='cuda')
+    small = torch.randn(2, nblk, hkv, page, d, generator=g).to(BF)
+    kc, vc = (room.as_strided((nblk, hkv, page, d), (hkv * d, d, stride, 1), i * nblk * hkv * d) for i in (0, 1))
+    kc.copy_(small[0]), vc.copy_(small[1])
+    tables = torch.tensor([[4, 1], [2, 3]] * rows, dtype=torch.int32)
+    common, past = torch.tensor([0, 5], dtype=torch.int32), torch.tensor([page, 2 * page - 2] * rows, dtype=torch.int32)
+    q = torch.randn(2 * rows, hq, d, generator=g).to(BF)
+    want, _, size = O.attention(q, *small, tables, past, common, 2 * page - 3, None, d ** -0.5)
+    got = IF.shared_prefix_attention(q.cuda(), kc, vc, tables.cuda(), past.cuda(), common.cuda(), 2 * page - 3)
+    near(got._t, want, O.attention_bound(want, size, BF))
+    qkv = torch.randn(2, (hq + 2) * d, generator=g).to(BF)
+    wq, wk, wv = O.append(qkv, *small, tables[:2], past[:2], None, None, False, 1.0)
+    IF.paged_rotary_append(qkv.cuda(), kc, vc, tables[:2].cuda(), past[:2].cuda())
+    assert torch.equal(kc.cpu().double(), wk) and torch.equal(vc.cpu().double(), wv)
