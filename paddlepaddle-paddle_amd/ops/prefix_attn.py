@@ -29,8 +29,8 @@ def _pages(cache, table, n):
     return torch.where(has[None, :, None], x, torch.zeros_like(x)), has
 
 
-def composite(q, key_cache, value_cache, tables, lens, ptable, plen, cu, scale):
-    """The definition, sequence by sequence, in 32 bits."""
+def composite(q, key_cache, value_cache, tables, lens, ptable, plen, cu, most, scale):
+    """The definition, sequence by sequence, in 32 bits; a sequence of more than ``most`` new tokens is NaN."""
     T, Hq, D = q.shape
     Hkv, page = key_cache.shape[1], key_cache.shape[2]
     G = Hq // Hkv
@@ -45,6 +45,9 @@ def composite(q, key_cache, value_cache, tables, lens, ptable, plen, cu, scale):
         vp, _ = _pages(value_cache, ptable, np_)
     for b in range(B):
         r0, n = c[b], c[b + 1] - c[b]
+        if n > most:
+            out[max(r0, 0):max(r0 + n, 0)] = lse[max(r0, 0):max(r0 + n, 0)] = float('nan')
+            continue
         if n <= 0 or r0 < 0 or r0 + n > T:
             continue
         L = max(0, min(int(lens[b]), tables.shape[1] * page))
@@ -93,9 +96,10 @@ def attend(q, key_cache, value_cache, tables, lens, ptable, plen, cu, most, scal
     T, Hq, D = q.shape
     nblk, Hkv, page, _ = key_cache.shape
     B = lens.shape[0]
+    most = max(1, min(most, T))
     if not supported(q, key_cache, value_cache):
         with torch.no_grad():
-            o, lse = composite(q, key_cache, value_cache, tables, lens, ptable, plen, cu, scale)
+            o, lse = composite(q, key_cache, value_cache, tables, lens, ptable, plen, cu, most, scale)
         return o, lse if want_lse else None
     out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=q.device) if want_lse else None
@@ -107,7 +111,6 @@ def attend(q, key_cache, value_cache, tables, lens, ptable, plen, cu, most, scal
     dev = isinstance(plen, torch.Tensor)
     cap = 0 if ptable is None else ptable.numel() * page
     plan = (ctypes.c_int * 5)()
-    most = max(1, min(most, T))
     N.check(N.lib.pa_prefix_attn_plan(T, B, Hq, Hkv, D, most, int(cu is not None), cap if dev else min(int(plen), cap),
                                       tables.shape[1] * page, plan), 'prefix_attn_plan')
     # this call's own workspace: two streams or two captured graphs never share one

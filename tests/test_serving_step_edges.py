@@ -73,3 +73,24 @@ def test_slot_strides_beyond_32_bits(page, stride, rows):
     wq, wk, wv = O.append(qkv, *small, tables[:2], past[:2], None, None, False, 1.0)
     IF.paged_rotary_append(qkv.cuda(), kc, vc, tables[:2].cuda(), past[:2].cuda())
     assert torch.equal(kc.cpu().double(), wk) and torch.equal(vc.cpu().double(), wv)
+
+
+# ------------------------------------------------------------------------------------------ what a call does not allow
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('d,dtype', [(64, BF), (128, HF), (64, FF), (80, BF)])   # kernel and composite
+def test_more_new_tokens_than_max_seqlen_q(dev, d, dtype):
+    """Rows of such a sequence are NaN, the others as ever; a row behind the last sequence is zero."""
+    g = torch.Generator().manual_seed(d)
+    n, own = [3, 2, 4, 0, 1], [5, 9, 4, 3, 20]
+    kc, vc, tables, common = paged(g, own, 16, 2, d, dtype, spare=2)
+    cu, lens = torch.tensor([0] + n).cumsum(0).int(), torch.tensor(own, dtype=torch.int32)
+    q = torch.randn(sum(n) + 2, 4, d, generator=g).to(dtype)
+    want, lse, size = O.attention(q, kc, vc, tables, lens, common, 20, cu, d ** -0.5)
+    args = [t.to(dev) for t in (q, kc, vc, tables, lens, common)]
+    out, l2 = (t._t.cpu() for t in IF.shared_prefix_attention(*args, 20, cu.to(dev), 2, return_lse=True))
+    over = torch.tensor([0, 1, 2, 5, 6, 7, 8])
+    fits = torch.tensor([3, 4, 9])
+    assert bool(out[over].isnan().all()) and bool(l2[over].isnan().all())
+    near(out[fits], want[fits], O.attention_bound(want, size, dtype)[fits])
+    near(l2[fits], lse[fits], 1e-3)
+    assert float(out[10:].float().abs().sum()) == 0.0 and bool((l2[10:] == -math.inf).all())
