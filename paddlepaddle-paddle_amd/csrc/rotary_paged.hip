@@ -192,7 +192,8 @@ struct AppendArgs {
   int max_blocks, num_blocks, page;
   const int* lens;  // tokens cached before this call
   const int* cu;    // [B + 1] or null: one token each
-  const int* off_dev;
+  const void* off_dev;  // int32 / int64 or null
+  int off64;
   long long off;  // position = off + place in the cache
   int T, B, Hq, Hkv, D, pairs, threads;
   float scale;
@@ -220,7 +221,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs A) {
             const int blk = A.tables[(long long)b * A.tstride + pg];
             if (blk >= 0 && blk < A.num_blocks) dst = blk * A.cs[0] + (p - pg * A.page) * A.cs[2];
           }
-          p += A.off_dev ? (long long)*A.off_dev : A.off;
+          p += !A.off_dev ? A.off
+                          : (A.off64 ? *reinterpret_cast<const int64_t*>(A.off_dev)
+                                     : (long long)*reinterpret_cast<const int32_t*>(A.off_dev));
           for (int i = threadIdx.x; i < A.pairs; i += A.threads) cs[i] = angle(A.inv_freq, A.scale, p, i, 1.f);
         }
         __syncthreads();
@@ -310,9 +313,9 @@ PA_API int pa_rope_freq(const void* q, const void* k, void* yq, void* yk, const 
 // The angle's position: off or *off_dev, + place.
 PA_API int pa_paged_append(const void* qkv, long long row, const void* bias, void* q, void* kc, void* vc,
                            const long long* cstr, const int* tables, long long tstride, int max_blocks, int num_blocks,
-                           int page, const int* lens, const int* cu, const int* off_dev, long long off, int T, int B,
-                           int Hq, int Hkv, int D, int pairs, int inter, const double* inv_freq, float scale,
-                           int align, int dt, hipStream_t st) {
+                           int page, const int* lens, const int* cu, const void* off_dev, int off64, long long off,
+                           int T, int B, int Hq, int Hkv, int D, int pairs, int inter, const double* inv_freq,
+                           float scale, int align, int dt, hipStream_t st) {
   if (T < 0 || B < 0 || Hq < 0 || Hkv <= 0 || D <= 0 || pairs < 0 || 2 * pairs > D || pairs > kMaxPairs || page <= 0 ||
       align < 1 || (pairs > 0 && !inv_freq))
     return (int)hipErrorInvalidValue;
@@ -321,7 +324,7 @@ PA_API int pa_paged_append(const void* qkv, long long row, const void* bias, voi
   A.qkv = qkv; A.row = row; A.bias = bias; A.q = q; A.kc = kc; A.vc = vc;
   for (int i = 0; i < 3; ++i) A.cs[i] = cstr[i];
   A.tables = tables; A.tstride = tstride; A.max_blocks = max_blocks; A.num_blocks = num_blocks; A.page = page;
-  A.lens = lens; A.cu = cu; A.off_dev = off_dev; A.off = off;
+  A.lens = lens; A.cu = cu; A.off_dev = off_dev; A.off64 = off64; A.off = off;
   A.T = T; A.B = B; A.Hq = Hq; A.Hkv = Hkv; A.D = D; A.pairs = pairs;
   A.inv_freq = inv_freq; A.scale = scale;
   const int v = width(dt == 0 ? 4 : 2, D, pairs, inter != 0, align);

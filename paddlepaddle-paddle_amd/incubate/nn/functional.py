@@ -938,12 +938,17 @@ def _same_device(name, first, **others):
             raise ValueError(f"{name}: {k} is on {t.device}, the input on {first.device}")
 
 
+def _narrow(t):
+    """int32 of an integer tensor; what does not fit becomes the end of the range, not a number of its low bits."""
+    return t if t.dtype == torch.int32 else t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
+
+
 def _int32(name, what, t, shape):
     t = _u(t)
     _check(isinstance(t, torch.Tensor) and t.dtype in (torch.int32, torch.int64), name, lambda: f"{what} must be an integer tensor")
     _check(t.dim() == len(shape) and all(n is None or n == m for n, m in zip(shape, t.shape)), name,
            lambda: f"{what} must have shape {list(shape)}, got {list(t.shape)}")
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return _narrow(t).contiguous()
 
 
 def _frequencies(name, inv_freq, D, interleaved):
@@ -1092,7 +1097,7 @@ def paged_rotary_append(qkv, key_cache, value_cache, block_tables, seq_lens, cu_
     off = _u(position_offset)
     if isinstance(off, torch.Tensor):
         _check(off.numel() == 1 and off.dtype in (torch.int32, torch.int64), name, "position_offset must be one integer")
-        off = off.reshape(1).to(torch.int32)
+        off = off.reshape(1)
     _same_device(name, t, key_cache=kc, value_cache=vc, block_tables=tables, seq_lens=lens, cu_seqlens_q=cu, inv_freq=f,
                  qkv_bias=bias, position_offset=off)
     q = ops.rotary_paged.paged_append(t, kc, vc, tables, lens, cu, f, bool(interleaved), float(attention_scale), bias, off)
@@ -1140,7 +1145,7 @@ def shared_prefix_attention(query, key_cache, value_cache, block_tables, seq_len
             pl = pt.numel() * kc.shape[2]
         elif isinstance(pl, torch.Tensor):
             _check(pl.numel() == 1 and pl.dtype in (torch.int32, torch.int64), name, "prefix_len must be one integer")
-            pl = pl.reshape(1).to(torch.int32)
+            pl = _narrow(pl.reshape(1))
         else:
             _check(0 <= int(pl) <= pt.numel() * kc.shape[2], name,
                    lambda: f"prefix_len {pl} does not fit {pt.numel()} blocks of {kc.shape[2]}")

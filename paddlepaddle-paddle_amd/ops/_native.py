@@ -171,7 +171,7 @@ _SIGS = {
     'pa_kv_cache_write': [I, P, P, LL, P, P, P, P, P, I, I, LL, P, P, I, I, I, P],
     'pa_kv_cache_write_q8': [I, I, P, P, LL, P, P, P, I, I, LL, P, P, I, I, I, P, P, LL, I, F, F, P],
     'pa_rope_freq': [P, P, P, P, LLP, LLP, I, I, I, I, I, I, I, P, F, P, LL, LL, I, F, I, I, P],
-    'pa_paged_append': [P, LL, P, P, P, P, LLP, P, LL, I, I, I, P, P, P, LL, I, I, I, I, I, I, I, P, F, I, I, P],
+    'pa_paged_append': [P, LL, P, P, P, P, LLP, P, LL, I, I, I, P, P, P, I, LL, I, I, I, I, I, I, I, P, F, I, I, P],
     'pa_prefix_attn_plan': [I, I, I, I, I, I, I, LL, LL, IP],
     'pa_prefix_attn': [P, P, P, LL, LL, LLP, P, LL, I, P, I, P, I, I, I, P, P, P, P, P, IP, I, I, I, I, I, I, F, I, P],
     'pa_sample_ws_bytes': [I],

@@ -135,7 +135,7 @@ def paged_append(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interl
             N.check(N.lib.pa_paged_append(
                 N.ptr(qkv), qkv.stride(0), N.ptr(bias), N.ptr(q), N.ptr(key_cache), N.ptr(value_cache),
                 _strides(key_cache), N.ptr(tables), tables.stride(0), tables.shape[1], nblk, page, N.ptr(lens), N.ptr(cu),
-                N.ptr(offset) if dev else None, 0 if dev else int(offset), T, B, Hq, Hkv, D, pairs, int(interleaved),
+                N.ptr(offset) if dev else None, int(dev and offset.dtype == torch.int64), 0 if dev else int(offset), T, B, Hq, Hkv, D, pairs, int(interleaved),
                 N.ptr(f), float(scale), a, N.dtcode(qkv.dtype), N.stream()), 'paged_append')
         return q
     with torch.no_grad():

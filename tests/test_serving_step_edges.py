@@ -94,3 +94,43 @@ def test_more_new_tokens_than_max_seqlen_q(dev, d, dtype):
     near(out[fits], want[fits], O.attention_bound(want, size, dtype)[fits])
     near(l2[fits], lse[fits], 1e-3)
     assert float(out[10:].float().abs().sum()) == 0.0 and bool((l2[10:] == -math.inf).all())
+
+
+# ------------------------------------------------------------------------------------------ 64-bit integers
+@pytest.mark.parametrize('dev', DEVICES)
+def test_integers_beyond_32_bits(dev):
+    """Blocks, lengths and offsets of 64 bits mean what they say: none comes back around as a small one."""
+    g = torch.Generator().manual_seed(12)
+    big, page, d = 1 << 32, 16, 64
+    kc, vc = (torch.randn(6, 1, page, d, generator=g).to(BF) for _ in range(2))
+    tables = torch.tensor([[0, 1], [2, 3], [4, 5]])
+    wild = torch.tensor([[0, 1], [2 + big, 3], [4, 5 - big]])                  # two blocks that are not the cache's
+    lens, f = torch.tensor([17, 5, 20]), frequencies(8)
+    qkv = torch.randn(3, 4 * d, generator=g).to(BF)
+    up = lambda t: t.to(dev)  # noqa: E731
+
+    def append(tables, lens, offset=0):
+        k, v = up(kc.clone()), up(vc.clone())
+        q = IF.paged_rotary_append(up(qkv), k, v, up(tables), up(lens), None, up(f), position_offset=offset)[0]
+        return q._t.cpu(), k.cpu(), v.cpu()
+    known = torch.tensor([[0, 1], [-1, 3], [4, -1]])
+    for a, b in zip(append(wild, lens), append(known, lens)):
+        assert torch.equal(a, b)
+    _, k, v = append(tables, torch.tensor([17, 5 + big, 20 - big]))            # places past the table and before it
+    _, k1, v1 = append(torch.tensor([[0, 1], [-1, -1], [-1, -1]]), lens)
+    assert torch.equal(k, k1) and torch.equal(v, v1)
+    # the length of a prefix before the positions; 1.3e10 radians in 64 bits are good to 3e-6 on either side
+    x, far = qkv.double().view(3, 4, d)[:, :2], 3 * big
+    for offset in (far, up(torch.tensor([far])), up(torch.tensor(7)), up(torch.tensor([7], dtype=torch.int32))):
+        want = O.rotate(x, lens + int(offset), f, False, 1.0)
+        near(append(tables, lens, offset)[0], want, O.rotate_bound(x, f, False, 1.0, BF) + 1e-5 * x.abs().amax())
+
+    def attend(tables, lens, prefix, plen, **kw):
+        return IF.shared_prefix_attention(up(qkv.view(3, 4, d)), up(kc), up(vc), up(tables), up(lens), up(prefix), plen, **kw)._t.cpu()
+    assert torch.equal(attend(wild, lens, torch.tensor([3, 1 + big]), 30), attend(known, lens, torch.tensor([3, -1]), 30))
+    assert torch.equal(attend(tables, torch.tensor([17 + big, 5, 20 - big]), torch.tensor([3]), up(torch.tensor(big + 2))),
+                       attend(tables, torch.tensor([32, 5, 0]), torch.tensor([3]), 16))
+    assert torch.equal(attend(tables, lens, torch.tensor([3]), up(torch.tensor(2 - big))), attend(tables, lens, torch.tensor([3]), 0))
+    # offsets of rows that do not fit the call: no sequence's
+    none = attend(tables, lens, torch.tensor([3]), 16, cu_seqlens_q=up(torch.tensor([0, 0, 3, 3]) + big), max_seqlen_q=3)
+    assert float(none.float().abs().sum()) == 0.0
