@@ -1018,13 +1018,14 @@ def fused_partial_rotary_embedding(q, k=None, inv_freq=None, position_ids=None, 
     integers [B, S], [1, S] or [S] ([T] for packed tokens), default 0 .. S - 1.  Pair i is (x[i], x[i + pairs]),
     or (x[2 i], x[2 i + 1]) with ``interleaved``; it is turned by position * inv_freq[i] and multiplied by
     ``attention_scale``.  Angles are formed in 64 bits, so positions may be far beyond a table's length, and no
-    table is built; both tensors take one kernel, and the gradient one more.  Returns (q, k), contiguous
-    (k None if not given)."""
+    table is built; both tensors take one kernel, and the gradient one more.  The frequencies are constants: ones
+    that ask for a gradient are refused.  Returns (q, k), contiguous (k None if not given)."""
     name = 'fused_partial_rotary_embedding'
     a, b = _u(q), _u(k) if k is not None else None
     _check(a.dim() in (3, 4), name, lambda: f"q must be [B, S, H, D] or [T, H, D], got {list(a.shape)}")
     _check(a.dtype in ops.rotary_paged.FLOATS, name, lambda: f"unsupported type {a.dtype}")
     f = _frequencies(name, inv_freq, a.shape[-1], interleaved)
+    _check(not (f.requires_grad and torch.is_grad_enabled()), name, "inv_freq has no gradient: detach it")
     _same_device(name, a, k=b, inv_freq=f, position_ids=_u(position_ids))
     if b is not None:
         _check(b.dtype == a.dtype, name, lambda: f"q is {a.dtype}, k {b.dtype}")

@@ -134,3 +134,21 @@ def test_integers_beyond_32_bits(dev):
     # offsets of rows that do not fit the call: no sequence's
     none = attend(tables, lens, torch.tensor([3]), 16, cu_seqlens_q=up(torch.tensor([0, 0, 3, 3]) + big), max_seqlen_q=3)
     assert float(none.float().abs().sum()) == 0.0
+
+
+# ------------------------------------------------------------------------------------------ what has a gradient
+@pytest.mark.parametrize('dev', DEVICES)
+def test_frequencies_that_want_a_gradient(dev):
+    """Frequencies are constants on every device: where a gradient would be lost the call is refused."""
+    x, f = torch.randn(1, 3, 2, 16, device=dev), frequencies(4).to(dev)
+    learned = f.clone().requires_grad_()
+    for q in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError, match='inv_freq'):
+            IF.fused_partial_rotary_embedding(q, q, learned)
+        want = IF.fused_partial_rotary_embedding(q, q, f)
+        for got in (IF.fused_partial_rotary_embedding(q, q, learned.detach()),):
+            assert all(torch.equal(a._t, b._t) for a, b in zip(got, want))
+    with torch.no_grad():
+        got = IF.fused_partial_rotary_embedding(x, None, learned)[0]
+    assert torch.equal(got._t, IF.fused_partial_rotary_embedding(x, None, f)[0]._t)
+    assert not got._t.requires_grad
