@@ -8,6 +8,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -78,16 +79,33 @@ def _launch(q, k, inv_freq, pos, interleaved, scale, sign):
     return yq, yk
 
 
+def _tangents():
+    """Whether tensors may carry tangents (forward-mode differentiation)."""
+    return forward_ad._current_level >= 0
+
+
 class _RopeFreq(torch.autograd.Function):
     """Linear in (q, k): the backward pass is the forward one with the angles' sign turned, so it has a
-    backward pass of its own."""
+    backward pass of its own, and a tangent is turned as its input is."""
 
     @staticmethod
     def forward(ctx, q, k, inv_freq, pos, interleaved, scale, sign):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(inv_freq, pos)
         ctx.how = (interleaved, scale, sign)
+        if _tangents():
+            ctx.save_for_forward(inv_freq, pos)
+            ctx.like = q, k
         return _launch(q, k, inv_freq, pos, interleaved, scale, sign)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        inv_freq, pos = ctx.saved_tensors
+        q, k = ctx.like
+        tq = torch.zeros_like(q) if tq is None else tq
+        tk = torch.zeros_like(k) if tk is None and k is not None else tk
+        ctx.like = None
+        return (_RopeFreq.apply if torch.is_grad_enabled() else _launch)(tq, tk, inv_freq, pos, *ctx.how)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -105,7 +123,7 @@ class _RopeFreq(torch.autograd.Function):
 def rope_freq(q, k, inv_freq, pos, interleaved, scale):
     """q [B, S, Hq, D], k [B, S, Hk, D] or None; inv_freq [pairs]; pos [B, S] integers or None (0 .. S - 1)."""
     if _hip(q):
-        wanted = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+        wanted = _tangents() or torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
         return (_RopeFreq.apply if wanted else _launch)(q, k, inv_freq, pos, interleaved, float(scale), 1.0)
     p = torch.arange(q.shape[1], device=q.device)[None] if pos is None else pos
     cos, sin = angles(p, inv_freq, scale)

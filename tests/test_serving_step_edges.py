@@ -152,3 +152,29 @@ def test_frequencies_that_want_a_gradient(dev):
         got = IF.fused_partial_rotary_embedding(x, None, learned)[0]
     assert torch.equal(got._t, IF.fused_partial_rotary_embedding(x, None, f)[0]._t)
     assert not got._t.requires_grad
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+def test_rotary_forward_mode(dev):
+    """The tangent of a rotation is the rotated tangent, whether the inputs want gradients or not."""
+    from torch.autograd import forward_ad
+    g = torch.Generator().manual_seed(13)
+    mk = lambda h: torch.randn(2, 5, h, 16, generator=g).to(dev)  # noqa: E731
+    f, (q, k, tq, tk) = frequencies(6).to(dev), (mk(3), mk(2), mk(3), mk(2))
+    turn = lambda q, k: [None if t is None else t._t for t in IF.fused_partial_rotary_embedding(q, k, f, interleaved=True)]  # noqa: E731
+    (wq, wk), (vq, vk) = turn(q, k), turn(tq, tk)
+    for wanted in (False, True):
+        q.requires_grad_(wanted), k.requires_grad_(wanted)
+        with forward_ad.dual_level():
+            for a, b, ta, tb in ((forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk), vq, vk),
+                                 (forward_ad.make_dual(q, tq), k, vq, None), (q, forward_ad.make_dual(k, tk), None, vk),
+                                 (forward_ad.make_dual(q, tq), None, vq, None)):
+                for out, want, tangent in zip(turn(a, b), (wq, wk), (ta, tb)):
+                    if out is None:
+                        continue
+                    got = forward_ad.unpack_dual(out)
+                    assert torch.equal(got.primal, want)
+                    if tangent is None:
+                        assert got.tangent is None or float(got.tangent.abs().max()) == 0.0
+                    else:
+                        assert torch.allclose(got.tangent, tangent, atol=1e-6)
