@@ -15,8 +15,10 @@
 // in flight while it computes on this one.  S^T = K Q^T on v_mfma_f32_16x16x32 (a lane holds 4 + 4 keys of
 // one row: maximum and sum take two lane swaps), P stays in registers as the B operand of O^T = V^T P^T,
 // whose A operand is V read transposed (ds_read_b64_tr_b16) in the matching key order.  P is rounded to
-// the inputs' type for that product, with a maximum that lags by at most 2^8 (no overflow in fp16), sums
-// and accumulators are 32-bit.  The NW parts are joined in LDS at the end.
+// the inputs' type for that product, sums and accumulators are 32-bit.  The base of the exponents lags behind the maximum
+// by at most 2^8, and in fp16 lies 2^7 under it: the largest probability is 2^15 at most, and what fp16 drops is 2^-32 of it
+// (with a largest of 1 it drops 2^-25, and thousands of keys behind one that takes nearly all are lost).  The NW parts are
+// joined in LDS at the end.
 //
 // Keys past the range and keys of unallocated pages (table entries outside the cache) are read from a row
 // of zeros and masked: what lies in a page's unused slots never reaches a product.
@@ -92,6 +94,9 @@ __device__ __forceinline__ void glds64(const void* src, unsigned lds_dst) {
       : "v"(src), "s"(lds_dst)
       : "memory");
 }
+
+template <typename T>
+constexpr float kUp = __is_same(T, f16_t) ? 7.f : 0.f;  // log2 of a probability whose score is the base's maximum
 
 // Weight of a part (m, l) in a join to maximum M.  A part that saw no key has m = -inf and l = 0; one whose
 // scores were all NaN has m = -inf and l = NaN, which has to reach the result.
@@ -228,7 +233,7 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
 
   f32x4 acc[RT][DB];            // O^T
   float l[RT];                  // sum of this lane's probabilities, before they are rounded
-  float nm[RT], thr[RT];        // minus the base of the exponents; the score at which it has to move
+  float nm[RT], thr[RT];        // minus the base of the exponents (the maximum - kUp); the score at which it has to move
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     nm[t] = 0.f;
@@ -374,9 +379,9 @@ __device__ __forceinline__ void item(const Args& A, char* smem, int hk, int tok0
       for (int t = 0; t < RT; ++t) {
         const float m1 = groups_max(mx[t]) * A.scale;
         const bool mv = m1 > thr[t];
-        const float f = thr[t] == -INFINITY ? 0.f : (mv ? fa::fast_exp2(-nm[t] - m1) : 1.f);
+        const float f = thr[t] == -INFINITY ? 0.f : (mv ? fa::fast_exp2(kUp<T> - nm[t] - m1) : 1.f);
         if (mv) {
-          nm[t] = -m1;
+          nm[t] = kUp<T> - m1;
           thr[t] = m1 + fa::kRescaleTau;
         }
         l[t] *= f;
@@ -694,9 +699,9 @@ __device__ __forceinline__ void wide_item(const Args& A, char* smem, int hk, int
       for (int t = 0; t < RT; ++t) {
         const float m1 = groups_max(mx[t]) * A.scale;
         const bool mv = m1 > thr[t];
-        const float f = thr[t] == -INFINITY ? 0.f : (mv ? fa::fast_exp2(-nm[t] - m1) : 1.f);
+        const float f = thr[t] == -INFINITY ? 0.f : (mv ? fa::fast_exp2(kUp<T> - nm[t] - m1) : 1.f);
         if (mv) {
-          nm[t] = -m1;
+          nm[t] = kUp<T> - m1;
           thr[t] = m1 + fa::kRescaleTau;
         }
         l[t] *= f;

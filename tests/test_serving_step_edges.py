@@ -178,3 +178,34 @@ def test_rotary_forward_mode(dev):
                         assert got.tangent is None or float(got.tangent.abs().max()) == 0.0
                     else:
                         assert torch.allclose(got.tangent, tangent, atol=1e-6)
+
+
+# ------------------------------------------------------------------------------------------ extreme scores
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('dtype', [BF, HF])
+@pytest.mark.parametrize('plen,rows', [(0, 2), (4000, 2), (4000, 80)])       # own keys, prefix items of few and of many rows
+def test_attention_behind_a_sink(dev, dtype, plen, rows):
+    """One key takes nearly all of the softmax and has no values; what the rows give comes from thousands of keys
+    that are each 2^-26 .. 2^-28 of it."""
+    g = torch.Generator().manual_seed(plen + rows)
+    own, d, page = 3000 if plen == 0 else 20, 64, 64
+    lens = torch.tensor([own] * rows, dtype=torch.int32)
+    kc, vc, tables, common = paged(g, [own], page, 1, d, dtype, spare=-(-plen // page))
+    tables = tables.expand(rows, -1).contiguous()
+    kc.zero_()
+    kc[..., 1] = torch.rand(kc.shape[:3], generator=g).to(dtype)             # scores in [-28, -26] times ln 2
+    kc[..., 0] = -26.0
+    vc.copy_((torch.rand(vc.shape, generator=g) * 20 + 40).to(dtype))
+    at = tables[0, 0] if plen == 0 else common[0]
+    kc[at, 0, 3], vc[at, 0, 3] = 0.0, 0.0
+    q = torch.zeros(rows, 2, d, dtype=dtype)
+    q[..., 0], q[..., 1] = 1.0, -2.0
+    scale = math.log(2)
+    want, lse, size = O.attention(q, kc, vc, tables, lens, common if plen else None, plen, None, scale)
+    got, l2 = IF.shared_prefix_attention(q.to(dev), kc.to(dev), vc.to(dev), tables.to(dev), lens.to(dev),
+                                         common.to(dev) if plen else None, plen if plen else None, scale=scale, return_lse=True)
+    assert float(want.min()) > 5e-4
+    # beside the rounding of normal numbers, in fp16 half the smallest step 2^-24 of a probability whose largest is 2^7
+    lost = (own + plen) * 2.0 ** -32 * 60 if dtype is HF else 0.0
+    near(got._t, want, O.attention_bound(want, size, dtype) + lost)
+    near(l2._t, lse, 1e-3)
