@@ -999,7 +999,11 @@ PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, i
     if (len <= 0) return 0;
     const long long cap = (len + 64 * nw - 1) / (64 * nw);  // two tiles a wave at least
     long long n = (target + items - 1) / items;
-    const long long least = (len + 8191) / 8192;            // no block walks more than 8192 keys alone
+    // No block walks more than 8192 keys alone, as long as the parts take no more than 1 GiB for it: `len` is what the
+    // table could hold, and with many new tokens a part for each 8192 keys of that would be more than there is
+    // (65536 tokens of 64 heads of 128 with tables for 2^20: 280 GB).  Many new tokens fill the chip by their rows.
+    const long long fits = (1ll << 28) / ((long long)T * Hq * (D + 2)), most_parts = fits < 1 ? 1 : fits;
+    const long long least = (len + 8191) / 8192 < most_parts ? (len + 8191) / 8192 : most_parts;
     if (n < least) n = least;
     return n < 1 ? 1 : (n > cap ? cap : n);
   };

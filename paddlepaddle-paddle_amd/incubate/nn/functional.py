@@ -1120,7 +1120,9 @@ def shared_prefix_attention(query, key_cache, value_cache, block_tables, seq_len
 
     Returns out [T, Hq, D], or (out, lse [T, Hq] float32) with ``return_lse``.  A token that sees no key, and a row
     behind the last sequence, is zero (lse -inf).  Keys in blocks that are not the cache's (-1) are not seen, lengths
-    past a table are cut to it, rows of a sequence with more than max_seqlen_q tokens are NaN.  The kernel takes
+    past a table are cut to it, rows of a sequence with more than max_seqlen_q tokens are NaN.  The work is cut by what
+    the tables could hold and by max_seqlen_q: tables not much wider than the longest sequence, and a max_seqlen_q that
+    is met, make a faster call.  The kernel takes
     float16 and bfloat16 with head dims 64, 128 and 256; other inputs take the composite of elementary operations,
     which waits for the device.  Inference only: no gradient flows."""
     name = 'shared_prefix_attention'

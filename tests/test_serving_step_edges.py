@@ -209,3 +209,47 @@ def test_attention_behind_a_sink(dev, dtype, plen, rows):
     lost = (own + plen) * 2.0 ** -32 * 60 if dtype is HF else 0.0
     near(got._t, want, O.attention_bound(want, size, dtype) + lost)
     near(l2._t, lse, 1e-3)
+
+
+# ------------------------------------------------------------------------------------------ tables wider than their sequences
+def plan(T, B, hq, hkv, d, most, packed, plen, own):
+    import ctypes
+    from paddle.ops import _native as N
+    if N._load() is None:
+        pytest.skip(N.load_error)
+    out = (ctypes.c_int * 5)()
+    N.check(N.lib.pa_prefix_attn_plan(T, B, hq, hkv, d, most, int(packed), plen, own, out), 'prefix_attn_plan')
+    return list(out)
+
+
+@pytest.mark.parametrize('T,B,hq,hkv,d,most', [(8192, 4, 64, 8, 128, 8192), (65536, 64, 64, 8, 128, 2048), (4096, 1, 16, 1, 256, 4096),
+                                               (300, 300, 64, 8, 128, 1), (32768, 8, 128, 1, 64, 32768)])
+def test_workspace_does_not_follow_the_tables(T, B, hq, hkv, d, most):
+    """Tables made for the longest length that is allowed, 2^20 tokens here, beside ones for 8192: at most 1 GiB of
+    partial results more."""
+    slot = T * hq * (d + 2) * 4
+    fits, wide = (plan(T, B, hq, hkv, d, most, most > 1, 5000, own)[4] for own in (8192, 1 << 20))
+    assert (wide - fits) * slot <= 1 << 30
+    assert wide >= fits
+
+
+@pytest.mark.gpu
+def test_chunks_with_wide_tables():
+    """The same chunks with tables that fit and with ones 100 times as wide: answers to the joins' rounding, memory to
+    1 GiB."""
+    g = torch.Generator().manual_seed(14)
+    own, n, hq, hkv, d, page = [2100, 900, 2048], [2048, 900, 1], 32, 2, 128, 64
+    kc, vc, tables, common = (t.cuda() for t in paged(g, own, page, hkv, d, BF, spare=2))
+    cu, lens = torch.tensor([0] + n).cumsum(0).int().cuda(), torch.tensor(own, dtype=torch.int32).cuda()
+    q = torch.randn(sum(n), hq, d, generator=g).to(BF).cuda()
+    wide = torch.nn.functional.pad(tables, (0, 100 * tables.shape[1]), value=-1)
+    outs, peaks = [], []
+    for t in (tables, wide):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        outs.append(IF.shared_prefix_attention(q, kc, vc, t, lens, common, cu_seqlens_q=cu, max_seqlen_q=2048)._t.double())
+        peaks.append(torch.cuda.max_memory_allocated() - before)
+    assert peaks[1] - peaks[0] <= 1 << 30
+    # 8 bits of each probability and of the result, on either side; values of normal size
+    assert float((outs[0] - outs[1]).abs().max()) <= 4 * 2.0 ** -8
