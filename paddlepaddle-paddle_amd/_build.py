@@ -9,7 +9,8 @@
   best-fit device allocator (host code over the HIP runtime, compiled with hipcc), loaded by
   torch's pluggable-allocator hook when enabled.
 
-Incremental: an object is rebuilt only when its source or a header is newer.
+Incremental: an object is rebuilt when its source or a header is newer or its flags are others than
+those it was built with, a library when one of its objects is newer or it was made of others.
 """
 import concurrent.futures
 import glob
@@ -24,6 +25,10 @@ OBJ = os.path.join(LIB, 'obj')
 ARCH = os.environ.get('PADDLE_AMD_ARCH', 'gfx950')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 
+# no packed fp32 instructions (v_pk_add/mul/fma_f32, which -O3 forms from ordinary float code): some of
+# their forms have given wrong results on this hardware
+FLAGS = ['-O3', '-fPIC', '-std=c++17', '-ffp-contract=fast', '-munsafe-fp-atomics',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 FILE_FLAGS = {
     # matrix instructions with vector-register accumulators: a wave of this kernel owns the whole register file, and
     # accumulators in its upper half are moved to the lower one and back in every turn of the key loop
@@ -42,6 +47,20 @@ def _newer(src, dst, deps=()):
     return any(os.path.getmtime(p) > t for p in (src, *deps))
 
 
+def _made_of(dst, what):
+    """Whether ``dst`` was last built from ``what`` (flags, parts), as the note beside it says."""
+    try:
+        with open(dst + '.made') as f:
+            return f.read() == '\n'.join(what)
+    except OSError:
+        return False
+
+
+def _note(dst, what):
+    with open(dst + '.made', 'w') as f:
+        f.write('\n'.join(what))
+
+
 def _run(cmd):
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
@@ -58,21 +77,25 @@ def build_kernels(verbose=False, jobs=None):
     for s in srcs:
         o = os.path.join(OBJ, os.path.basename(s) + '.o')
         objs.append(o)
-        if _newer(s, o, headers):
-            todo.append((s, o))
-    # no packed fp32 instructions (v_pk_add/mul/fma_f32, which -O3 forms from ordinary float code): some of
-    # their forms have given wrong results on this hardware
-    cmds = [[HIPCC, '-O3', f'--offload-arch={ARCH}', '-fPIC', '-std=c++17', '-ffp-contract=fast', '-munsafe-fp-atomics',
-             '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '-I', CSRC, '-c', s, '-o', o]
-            + FILE_FLAGS.get(os.path.basename(s), []) for s, o in todo]
+        flags = [f'--offload-arch={ARCH}', *FLAGS, *FILE_FLAGS.get(os.path.basename(s), [])]
+        if _newer(s, o, headers) or not _made_of(o, flags):
+            todo.append((s, o, flags))
+
+    def compile_one(s, o, flags):
+        out = _run([HIPCC, *flags, '-I', CSRC, '-c', s, '-o', o])
+        _note(o, flags)
+        return out
     jobs = jobs or min(8, os.cpu_count() or 4)
     with concurrent.futures.ThreadPoolExecutor(jobs) as ex:
-        for out in ex.map(_run, cmds):
+        for out in ex.map(lambda t: compile_one(*t), todo):
             if verbose and out.strip():
                 print(out)
-    if todo or not os.path.exists(KERNEL_LIB) or any(os.path.getmtime(o) > os.path.getmtime(KERNEL_LIB) for o in objs):
+    parts = [os.path.basename(o) for o in objs]
+    if (todo or not os.path.exists(KERNEL_LIB) or any(os.path.getmtime(o) > os.path.getmtime(KERNEL_LIB) for o in objs)
+            or not _made_of(KERNEL_LIB, parts)):
         _run([HIPCC, f'--offload-arch={ARCH}', '-shared', '-fPIC', '-o', KERNEL_LIB + '.tmp', *objs])
         os.replace(KERNEL_LIB + '.tmp', KERNEL_LIB)
+        _note(KERNEL_LIB, parts)
     return KERNEL_LIB
 
 
