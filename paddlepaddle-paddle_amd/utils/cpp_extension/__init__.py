@@ -6,6 +6,9 @@ Custom operators are built for gfx950 with hipcc:
   with ``--offload-arch=gfx950``), built in-tree under ``get_build_directory()``;
 * ``load_hip_library(name, sources)`` — plain C-ABI ``extern "C"`` launchers (the way this
   framework's own kernels are built), returned as a ctypes library.
+
+HIP sources are compiled without packed fp32 instructions (v_pk_add/mul/fma_f32, which -O3 forms from ordinary
+float code): some of their forms have given wrong results on this hardware.
 """
 import ctypes
 import hashlib
@@ -13,6 +16,9 @@ import os
 import subprocess
 
 _BUILD = os.environ.get('PADDLE_EXTENSION_DIR', os.path.join(os.getcwd(), '.paddle_extensions'))
+
+
+_NO_PACKED = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def get_build_directory(verbose=False):
@@ -31,7 +37,7 @@ def load(name, sources, extra_cxx_cflags=None, extra_cuda_cflags=None, extra_ldf
     bdir = build_directory or os.path.join(get_build_directory(), name)
     os.makedirs(bdir, exist_ok=True)
     return tce.load(name=name, sources=list(sources), extra_cflags=extra_cxx_cflags or [],
-                    extra_cuda_cflags=(extra_cuda_cflags or []) + [f'--offload-arch={_arch()}'],
+                    extra_cuda_cflags=(extra_cuda_cflags or []) + [f'--offload-arch={_arch()}', *_NO_PACKED],
                     extra_ldflags=extra_ldflags or [], extra_include_paths=extra_include_paths or [],
                     build_directory=bdir, verbose=verbose)
 
@@ -44,11 +50,12 @@ def load_hip_library(name, sources, extra_cflags=None, build_directory=None):
     for s in sources:
         with open(s, 'rb') as f:
             h.update(f.read())
-    h.update(' '.join(extra_cflags or []).encode())
+    flags = [*_NO_PACKED, *(extra_cflags or [])]
+    h.update(' '.join(flags).encode())
     out = os.path.join(bdir, f"lib{name}_{h.hexdigest()[:10]}.so")
     if not os.path.exists(out):
         hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-        cmd = [hipcc, '-O3', f'--offload-arch={_arch()}', '-fPIC', '-shared', '-std=c++17', *(extra_cflags or []),
+        cmd = [hipcc, '-O3', f'--offload-arch={_arch()}', '-fPIC', '-shared', '-std=c++17', *flags,
                *sources, '-o', out + '.tmp']
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
@@ -65,6 +72,10 @@ def CppExtension(sources, *args, **kwargs):  # noqa: N802
 def CUDAExtension(sources, *args, **kwargs):  # noqa: N802
     os.environ.setdefault('PYTORCH_ROCM_ARCH', _arch())
     from torch.utils import cpp_extension as tce
+    flags = kwargs.get('extra_compile_args') or {}
+    flags = dict(flags) if isinstance(flags, dict) else {'cxx': list(flags), 'nvcc': list(flags)}
+    flags['nvcc'] = [*flags.get('nvcc', []), *_NO_PACKED]
+    kwargs['extra_compile_args'] = flags
     return tce.CUDAExtension(kwargs.pop('name', 'paddle_custom_ops'), sources, *args, **kwargs)
 
 

@@ -66,3 +66,30 @@ def test_kernels_have_no_packed_fp32(build):
     _, compiled = build
     for line in compiled()[2]:
         assert ' -shared ' in line or '-Xclang -target-feature -Xclang -packed-fp32-ops' in line
+
+
+def test_custom_operators_have_no_packed_fp32(tmp_path, monkeypatch):
+    """A user's own kernels get the flag too, by each of the ways to build them."""
+    from paddle.utils import cpp_extension as X
+    log, cc, src = tmp_path / 'log', tmp_path / 'cc', tmp_path / 'k.hip'
+    cc.write_text(f'#!/bin/sh\necho "$@" >> {log}\nexec /opt/rocm/bin/hipcc "$@"\n')
+    cc.chmod(cc.stat().st_mode | stat.S_IXUSR)
+    src.write_text('#include <hip/hip_runtime.h>\n__global__ void k(float2* x) { x[threadIdx.x].x *= 2; x[threadIdx.x].y *= 3; }\n'
+                   'extern "C" int answer() { return 42; }\n')
+    monkeypatch.setenv('HIPCC', str(cc))
+    lib = X.load_hip_library('t', [str(src)], extra_cflags=['-DA=1'], build_directory=str(tmp_path / 'b'))
+    assert lib.answer() == 42
+    args = log.read_text().split()
+    at = args.index('-packed-fp32-ops')
+    assert args[at - 3:at] == ['-Xclang', '-target-feature', '-Xclang'] and '-DA=1' in args
+    seen = {}
+    from torch.utils import cpp_extension as tce
+    monkeypatch.setattr(tce, 'load', lambda **kw: seen.update(kw))
+    X.load('t', [str(src)], extra_cuda_cflags=['-DB'], build_directory=str(tmp_path / 'c'))
+    assert '-packed-fp32-ops' in seen['extra_cuda_cflags'] and '-DB' in seen['extra_cuda_cflags']
+    monkeypatch.setattr(tce, 'CUDAExtension', lambda name, sources, *a, **kw: kw)
+    for given in (None, ['-DC'], {'cxx': ['-DC']}, {'nvcc': ['-DC']}):
+        got = X.CUDAExtension([str(src)], **({} if given is None else dict(extra_compile_args=given)))['extra_compile_args']
+        assert '-packed-fp32-ops' in got['nvcc'] and '-packed-fp32-ops' not in got.get('cxx', [])
+        if given is not None:
+            assert all('-DC' in got[k] for k in (('cxx', 'nvcc') if isinstance(given, list) else given))
