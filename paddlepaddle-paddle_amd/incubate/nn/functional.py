@@ -1157,7 +1157,7 @@ def shared_prefix_attention(query, key_cache, value_cache, block_tables, seq_len
                "prefix_len without prefix_blocks")
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     _check(scale > 0 and math.isfinite(scale), name, lambda: f"scale must be positive and finite, got {scale}")
-    aligned = kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in kc.stride()[:3])
+    aligned = kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0 and all(s % 8 == 0 or n == 1 for s, n in zip(kc.stride()[:3], kc.shape))
     _check(aligned or not ops.prefix_attn.supported(q, kc, vc), name, "caches need 16-byte aligned rows")
     _same_device(name, q, key_cache=kc, value_cache=vc, block_tables=tables, seq_lens=lens, cu_seqlens_q=cu,
                  prefix_blocks=pt, prefix_len=pl)

@@ -253,3 +253,17 @@ def test_chunks_with_wide_tables():
     assert peaks[1] - peaks[0] <= 1 << 30
     # 8 bits of each probability and of the result, on either side; values of normal size
     assert float((outs[0] - outs[1]).abs().max()) <= 4 * 2.0 ** -8
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+def test_strides_of_one_head(dev):
+    """A dimension of size 1 has no stride that matters: caches of one key head (or of pages of one place, or of one
+    block) that differ from contiguous ones in nothing else are taken as they are."""
+    g = torch.Generator().manual_seed(15)
+    for nblk, page, odd in ((5, 16, (16 * 64, 3, 64, 1)), (5, 1, (64, 64, 7, 1)), (1, 16, (5, 64, 64, 1))):
+        kc, vc = (torch.randn(nblk, 1, page, 64, generator=g).to(BF).to(dev) for _ in range(2))
+        q = torch.randn(1, 4, 64, generator=g).to(BF).to(dev)
+        tables, lens = torch.arange(nblk, dtype=torch.int32)[None].to(dev), torch.tensor([nblk * page], dtype=torch.int32).to(dev)
+        want = IF.shared_prefix_attention(q, kc, vc, tables, lens)
+        got = IF.shared_prefix_attention(q, kc.as_strided(kc.shape, odd), vc.as_strided(vc.shape, odd), tables, lens)
+        assert torch.equal(got._t, want._t)
