@@ -34,6 +34,11 @@ def _alignment(ts):
     return a
 
 
+def _even(t):
+    """t, copied where its address or a stride is odd (contiguous() leaves a view at an odd address as it is)."""
+    return t if t is None or _alignment((t,)) % 2 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def _strides(t):
     return (ctypes.c_longlong * 3)(*t.stride()[:3])
 
@@ -64,7 +69,7 @@ def _launch(q, k, inv_freq, pos, interleaved, scale, sign):
         k = k.contiguous()
     a = _alignment((q, k))
     if interleaved and a % 2:
-        q, k = q.contiguous(), None if k is None else k.contiguous()
+        q, k = _even(q), _even(k)
         a = _alignment((q, k))
     yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
@@ -143,8 +148,7 @@ def paged_append(qkv, key_cache, value_cache, tables, lens, cu, inv_freq, interl
         if interleaved and a % 2:
             if _alignment((key_cache, value_cache)) % 2:
                 raise ValueError("interleaved pairs need caches of even strides")
-            qkv = qkv.contiguous()
-            bias = None if bias is None or _alignment((bias,)) % 2 == 0 else bias.clone()
+            qkv, bias = _even(qkv), _even(bias)
             a = _alignment((qkv, key_cache, value_cache, bias))
         q = torch.empty(T, Hq, D, dtype=qkv.dtype, device=qkv.device)
         f = None if inv_freq is None else inv_freq.double().contiguous()

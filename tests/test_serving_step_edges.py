@@ -267,3 +267,28 @@ def test_strides_of_one_head(dev):
         want = IF.shared_prefix_attention(q, kc, vc, tables, lens)
         got = IF.shared_prefix_attention(q, kc.as_strided(kc.shape, odd), vc.as_strided(vc.shape, odd), tables, lens)
         assert torch.equal(got._t, want._t)
+
+
+@pytest.mark.parametrize('dev', DEVICES)
+@pytest.mark.parametrize('dtype', [BF, FF])
+def test_interleaved_pairs_at_odd_addresses(dev, dtype):
+    """Contiguous views that begin at an odd element: pairs are loaded together, so they are copied first."""
+    g = torch.Generator().manual_seed(16)
+    f, odd = frequencies(8).to(dev), lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)  # noqa: E731
+    q, k, gq, gk = (torch.randn(1, 3, h, 16, generator=g).to(dtype).to(dev) for h in (3, 2, 3, 2))
+    leaves = [t.clone().requires_grad_() for t in (q, k)]
+
+    def both(q, k, gq, gk):
+        y = [t._t for t in IF.fused_partial_rotary_embedding(q, k, f, interleaved=True)]
+        return [t.detach() for t in y] + list(torch.autograd.grad(y, [q, k], [gq, gk]))
+    want = both(*leaves, gq, gk)
+    got = both(*(odd(t).detach().requires_grad_() for t in (q, k)), odd(gq), odd(gk))
+    assert odd(q).data_ptr() % (2 * q.element_size()) and odd(q).is_contiguous()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    qkv, bias = torch.randn(1, 4 * 16, generator=g).to(dtype).to(dev), torch.randn(64, generator=g).to(dtype).to(dev)
+    table, lens = torch.tensor([[1, 0]], dtype=torch.int32).to(dev), torch.tensor([5], dtype=torch.int32).to(dev)
+    outs = []
+    for x, b in ((qkv, bias), (odd(qkv), bias), (qkv, odd(bias)), (odd(qkv), odd(bias))):
+        kc, vc = (torch.zeros(2, 1, 4, 16, dtype=dtype, device=dev) for _ in range(2))
+        outs.append((IF.paged_rotary_append(x, kc, vc, table, lens, None, f, True, qkv_bias=b)[0]._t, kc, vc))
+        assert all(torch.equal(a, c) for a, c in zip(outs[-1], outs[0]))
