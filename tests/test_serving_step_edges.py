@@ -292,3 +292,41 @@ def test_interleaved_pairs_at_odd_addresses(dev, dtype):
         kc, vc = (torch.zeros(2, 1, 4, 16, dtype=dtype, device=dev) for _ in range(2))
         outs.append((IF.paged_rotary_append(x, kc, vc, table, lens, None, f, True, qkv_bias=b)[0]._t, kc, vc))
         assert all(torch.equal(a, c) for a, c in zip(outs[-1], outs[0]))
+
+
+# ------------------------------------------------------------------------------------------ scaled frequencies
+@pytest.mark.parametrize('rot,base,span,factor', [(64, 10000.0, 4096, 8.0), (128, 500000.0, 8192, 32.0), (32, 100.0, 64, 3.0)])
+@pytest.mark.parametrize('bounds', [None, (2.0, 16.0)])
+def test_scaled_frequencies_pair_by_pair(rot, base, span, factor, bounds):
+    """Every pair by its own formula, the blended ones between the kept and the divided ones among them."""
+    plain = [base ** (-2.0 * i / rot) for i in range(rot // 2)]
+    lo, hi = bounds or (1.0, 4.0)
+    want, blended = [], 0
+    for f in plain:
+        wavelength = 2 * math.pi / f
+        if wavelength < span / hi:
+            want.append(f)
+        elif wavelength > span / lo:
+            want.append(f / factor)
+        else:
+            part = (span / wavelength - lo) / (hi - lo)
+            want.append((1 - part) * f / factor + part * f)
+            blended += 1
+    more = {} if bounds is None else dict(low_freq_factor=lo, high_freq_factor=hi)
+    got, s = IF.rotary_inv_freq(rot, base, dict(type='wavelength', factor=factor, original_max_position=span, **more))
+    assert blended > 0 and s == 1.0
+    assert all(math.isclose(a, b, rel_tol=1e-12) for a, b in zip(got._t.tolist(), want, strict=True))
+    # the pair that makes `turns` turns over the span: base ** (-2 i / rot) * span = 2 pi turns, solved for i
+    slow, fast = bounds or (1.0, 32.0)
+    at = lambda turns: rot * math.log(span / (2 * math.pi * turns)) / (2 * math.log(base))  # noqa: E731
+    first, last = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rot - 1)
+    want = []
+    for i, f in enumerate(plain):
+        part = min(max((i - first) / max(last - first, 1e-3), 0.0), 1.0)
+        want.append(f * (1 - part) + f / factor * part)
+    more = {} if bounds is None else dict(beta_slow=slow, beta_fast=fast)
+    got, s = IF.rotary_inv_freq(rot, base, dict(type='yarn', factor=factor, original_max_position=span, **more))
+    assert any(1 < a / b < factor for a, b in zip(plain, want))
+    assert all(math.isclose(a, b, rel_tol=1e-12) for a, b in zip(got._t.tolist(), want, strict=True))
+    assert math.isclose(s, 0.1 * math.log(factor) + 1, rel_tol=1e-12)
+    assert IF.rotary_inv_freq(rot, base, dict(type='yarn', factor=factor, original_max_position=span, attention_factor=0.75))[1] == 0.75
