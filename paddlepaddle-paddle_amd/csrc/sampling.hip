@@ -469,11 +469,12 @@ __device__ __forceinline__ bool vector_rows(const Args& A) {
   return (reinterpret_cast<uintptr_t>(A.x) & 15) == 0 && A.row % (16 / (int)sizeof(T)) == 0;
 }
 
-// What bounds it: 64-bit arithmetic, some 13 operations a token (a 32-bit mass would move the borders).  64 rows of
-// 128256 tokens in bf16 17 us, 512 rows of 32000 in fp32 27 us (2.4 TB/s), one row of 50304 8 us.  With one atomic for
-// count and mass instead of two, and with four copies of the bins, a twentieth less: the atomics are not what it waits
-// for.  Lists of a chunk's largest 128 tokens, written here, save the row's block 16 of 50 us at 128256 tokens and cost
-// 6 here, and at 32000 they cost 8 and save none: the row's block looks the tokens up by the maxima of parts instead.
+// What bounds it: vector instructions, 38 a token of which some 13 are 64-bit (a 32-bit mass would move the borders): their
+// issue takes half of the time; the LDS a fifth, more than half of that in bank conflicts of the bins.  64 rows of 128256
+// tokens in bf16 17 us, 512 rows of 32000 in fp32 27 us (2.4 TB/s), one row of 50304 8 us.  With one atomic for count and
+// mass instead of two, and with four copies of the bins, a twentieth less.  Lists of a chunk's largest 128 tokens, written
+// here, save the row's block 16 of 50 us at 128256 tokens and cost 6 here, and at 32000 they cost 8 and save none: the
+// row's block looks the tokens up by the maxima of parts at every size.
 template <typename T>
 __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ out, int nc) {
   const int r = blockIdx.x / nc, ch = blockIdx.x % nc, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -564,7 +565,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args A, Chunk* __restrict__ 
 
 // Bounded by latency: some ten dependent steps over a few KB, one re-read of the parts that have a border's tokens, and
 // one chunk's scan.  One row of 50304 tokens 18 us (4 the first loads, 3 the join of the histograms, 5 the list, 1 each
-// selection); 64 rows of 128256 38 .. 45 us, as their longest list is; 512 rows of 32000 41 us.
+// selection); 64 rows of 128256 37 .. 45 us, as their longest list is; 512 rows of 32000 40 .. 43 us.
 template <typename T>
 __global__ __launch_bounds__(NT, 4) void row_kernel(Args A, const Chunk* __restrict__ in, int nc) {
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
