@@ -989,7 +989,7 @@ static int pfx_rto(long long rows, int D) { return rows <= 16 ? 1 : (D == 256 ? 
 // lengths are on the device).
 PA_API int pa_prefix_attn_plan(int T, int B, int Hq, int Hkv, int D, int most, int packed, long long plen,
                                 long long own, int* out) {
-  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || most <= 0 || (D != 64 && D != 128 && D != 256))
+  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || most <= 0 || (D != 64 && D != 128 && D != 256))
     return (int)hipErrorInvalidValue;
   const long long G = Hq / Hkv, nw = pfx_nw(D);
   const int rtp = pfx_rtp((long long)T * G, D), rto = pfx_rto(most * G, D);
@@ -1035,7 +1035,7 @@ PA_API int pa_prefix_attn(const void* q, const void* kc, const void* vc, long lo
                           const int* lens, const int* cu, void* out, float* lse, float* ws,
                           const int* plan, int T, int B, int Hq, int Hkv, int D, int most, float scale, int dt,
                           hipStream_t st) {
-  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || page <= 0 || num_blocks < 0 || (dt != 1 && dt != 2) ||
+  if (T <= 0 || B <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || page <= 0 || num_blocks < 0 || (dt != 1 && dt != 2) ||
       !(scale > 0.f) || cstr[2] < 0 || (!cu && T != B) || (plan[4] > 0 && !ws))
     return (int)hipErrorInvalidValue;
   Args A;

@@ -330,3 +330,9 @@ def test_scaled_frequencies_pair_by_pair(rot, base, span, factor, bounds):
     assert all(math.isclose(a, b, rel_tol=1e-12) for a, b in zip(got._t.tolist(), want, strict=True))
     assert math.isclose(s, 0.1 * math.log(factor) + 1, rel_tol=1e-12)
     assert IF.rotary_inv_freq(rot, base, dict(type='yarn', factor=factor, original_max_position=span, attention_factor=0.75))[1] == 0.75
+
+
+def test_plan_refuses_calls_without_heads():
+    """An error code, not a division by zero."""
+    with pytest.raises(RuntimeError):
+        plan(4, 4, 0, 2, 64, 1, False, 0, 64)
